@@ -1,0 +1,380 @@
+"""The language-model training operators as measurable cases: embedding lookup with scaling and its
+gradient, residual norms (before / after a block, with gate and residual scale), and the global
+gradient norm with clipping.
+
+``own = False`` computes the formulas with elementary torch operations in fp32, rounded once at the
+end; ``own = True`` makes the calls a user makes of the framework.  Inputs are made from the seed
+alone, on the GPU.
+"""
+import itertools
+import math
+import random
+
+import torch
+
+own = False
+
+_TYPES = {"float32": torch.float32, "bfloat16": torch.bfloat16, "float16": torch.float16,
+          "int64": torch.int64, "int32": torch.int32}
+_BYTES = {"float32": 4, "bfloat16": 2, "float16": 2, "int64": 8, "int32": 4}
+_LR, _MOMENTUM, _DECAY = 0.01, 0.9, 0.01
+
+
+def listed():
+    return [
+        # --- embedding
+        # a serving step: one new token for each of 8 sequences, 16-bit table; latency counts
+        dict(name="embed 8 tokens", op="embed", batch=8, length=1, vocab=30522, width=768, table="bfloat16",
+             out="bfloat16", index="int64", scale=1.0, pad=False, train=False),
+        # one step of the LSTM language model: 35 x 20 tokens, odd width
+        dict(name="embed lstm step", op="embed", batch=35, length=20, vocab=10000, width=650, table="float32",
+             out="float32", index="int64", scale=1.0, pad=False, train=True),
+        # one step of the encoder: 32 sequences of 128 tokens, an eighth of them the mask token, padded tails
+        dict(name="embed encoder step", op="embed", batch=32, length=128, vocab=30522, width=768, table="float32",
+             out="float32", index="int64", scale=1.0, pad=True, train=True),
+        # a long-context step: 64 x 1024 tokens, scaled by sqrt(width), fp32 table, 16-bit activations
+        dict(name="embed long batch", op="embed", batch=64, length=1024, vocab=50001, width=1024, table="float32",
+             out="bfloat16", index="int32", scale=32.0, pad=True, train=True),
+        # --- norms around a block
+        # one token of 4 sequences between two blocks while serving; latency counts
+        dict(name="norm 4 tokens", op="norm", batch=4, length=1, width=768, stream="bfloat16", block="bfloat16",
+             kind="layer", post=False, gate="none", alpha=1.0, bias=True, train=False),
+        # after a block of the encoder: norm(x + f(x)), fp32, with its backward
+        dict(name="norm encoder step", op="norm", batch=32, length=128, width=768, stream="float32", block="float32",
+             kind="layer", post=False, gate="none", alpha=1.0, bias=True, train=True),
+        # the width of the LSTM, ragged rows, a gate for each channel and a residual scale, 16-bit
+        dict(name="norm odd width", op="norm", batch=35, length=21, width=651, stream="float16", block="float16",
+             kind="layer", post=False, gate="channel", alpha=1.5, bias=True, train=True),
+        # long sequences: norm after the block, gate for each sample, norm before the next block
+        dict(name="norm gated long", op="norm", batch=16, length=2048, width=4096, stream="bfloat16",
+             block="bfloat16", kind="rms", post=True, gate="sample", alpha=1.0, bias=False, train=True),
+        # --- global norm and clipping
+        # a small model's ten tensors, norm under the bound: latency counts
+        dict(name="clip small", op="clip", tensors="lstm", vocab=500, width=64, grads="float32", bound=2.0,
+             packed=False),
+        # the LSTM's gradients; the ordinary step leaves them as they are
+        dict(name="clip lstm", op="clip", tensors="lstm", vocab=10000, width=650, grads="float32", bound=2.0,
+             packed=False),
+        # the encoder's two hundred tensors, 16-bit gradients
+        dict(name="clip encoder", op="clip", tensors="encoder", vocab=30522, width=768, grads="bfloat16", bound=2.0,
+             packed=False),
+        # the encoder's update with clipped gradients: norm, scale, momentum, weights
+        dict(name="clipped step encoder", op="step", tensors="encoder", vocab=30522, width=768, grads="float32",
+             bound=0.5, packed=False),
+    ]
+
+
+def _log(rng, lo, hi):
+    return int(round(math.exp(rng.uniform(math.log(lo), math.log(hi)))))
+
+
+def draw(rng):
+    op = rng.choice(("embed", "norm", "clip", "step"))
+    if op == "embed":
+        width = _log(rng, 1, 4096)
+        vocab = min(_log(rng, 2, 100000), 50001 * 1024 // width)
+        tokens = max(1, min(_log(rng, 1, 131072), 65536 * 1024 // width))
+        batch = rng.choice((1, 2, 5, 16, 35))
+        kind = rng.choice(("float32", "float32", "bfloat16", "float16"))
+        return dict(op=op, batch=batch, length=max(1, tokens // batch), vocab=vocab, width=width, table=kind,
+                    out=rng.choice((kind, "bfloat16")), index=rng.choice(("int64", "int32")),
+                    scale=rng.choice((1.0, round(math.sqrt(width), 4))), pad=rng.random() < 0.5,
+                    train=rng.random() < 0.75)
+    if op == "norm":
+        width = _log(rng, 32, 12000)
+        rows = max(1, min(_log(rng, 1, 32768), 32768 * 4096 // width))
+        batch = rng.choice((1, 2, 5, 16, 35))
+        stream = rng.choice(("float32", "bfloat16", "float16"))
+        block = rng.choice(("float32", "bfloat16", "float16")) if stream == "float32" else stream
+        return dict(op=op, batch=batch, length=max(1, rows // batch), width=width, stream=stream, block=block,
+                    kind=rng.choice(("layer", "rms")), post=rng.random() < 0.4,
+                    gate=rng.choice(("none", "channel", "sample", "full")), alpha=rng.choice((1.0, 1.5, 0.7)),
+                    bias=rng.random() < 0.5, train=rng.random() < 0.75)
+    grads = "float32" if op == "step" else rng.choice(("float32", "bfloat16", "float16"))
+    return dict(op=op, tensors="ragged", count=_log(rng, 1, 400), most=_log(rng, 16, 2000000),
+                shapes=rng.randrange(1 << 20), grads=grads, bound=rng.choice((0.5, 2.0)), packed=rng.random() < 0.5)
+
+
+def _sizes(case):
+    """The element counts of the tensors, as the models lay them out."""
+    if case["tensors"] == "ragged":
+        r = random.Random(case["shapes"])
+        return [_log(r, 1, case["most"]) for _ in range(case["count"])]
+    v, d = case["vocab"], case["width"]
+    if case["tensors"] == "lstm":
+        return [v * d] + [4 * d * d, 4 * d * d, 4 * d, 4 * d] * 2 + [v * d, v]
+    layer = [3 * d * d, 3 * d, d * d, d, d, d, 4 * d * d, 4 * d, 4 * d * d, d, d, d]
+    return [v * d, 512 * d, 2 * d, d, d] + layer * 12 + [d * d, d, d, d, v]
+
+
+def _places(case):
+    """(offset, size) of each tensor in its flat buffer: 64-element places, as an allocator gives
+    them, or packed end to end, as gradients in a bucket lie."""
+    sizes = _sizes(case)
+    ends = list(itertools.accumulate(n if case["packed"] else -(-n // 64) * 64 for n in sizes))
+    return list(zip([0] + ends[:-1], sizes)), ends[-1]
+
+
+def _views(case, flat):
+    return [flat[at:at + n] for at, n in _places(case)[0]]
+
+
+def prepare(case, seed):
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+
+    def normal(*shape, dtype="float32", scale=1.0, mean=0.0):
+        return torch.randn(*shape, generator=gen, device="cuda").mul_(scale).add_(mean).to(_TYPES[dtype])
+
+    if case["op"] == "embed":
+        b, t, v, d = case["batch"], case["length"], case["vocab"], case["width"]
+        # token frequencies fall with the rank (density 1 / rank); row 0 is padding, an eighth is one mask token
+        u = torch.rand(b, t, generator=gen, device="cuda")
+        ids = torch.exp(u.double() * math.log(v)).long().clamp_(1, v) - 1
+        if case["train"]:
+            ids[torch.rand(b, t, generator=gen, device="cuda") < 0.125] = min(103, v - 1)
+        if case["pad"]:
+            full = torch.randint(1, t + 1, (b, 1), generator=gen, device="cuda")
+            ids[torch.arange(t, device="cuda")[None] >= full.clamp_(min=t // 2)] = 0
+        state = dict(case=case, ids=ids.to(_TYPES[case["index"]]), weight=normal(v, d, dtype=case["table"], scale=0.02))
+        if case["train"]:
+            state["dy"] = normal(b, t, d, dtype=case["out"], scale=0.01)
+        return state
+    if case["op"] == "norm":
+        b, t, d = case["batch"], case["length"], case["width"]
+        state = dict(case=case, x=normal(b, t, d, dtype=case["stream"], mean=0.1),
+                     y=normal(b, t, d, dtype=case["block"], scale=0.5),
+                     weight=normal(d, scale=0.1, mean=1.0), bias=normal(d, scale=0.1) if case["bias"] else None)
+        shape = {"none": None, "channel": (d,), "sample": (b, 1, d), "full": (b, t, d)}[case["gate"]]
+        state["gate"] = normal(*shape, dtype=case["block"], scale=0.3, mean=0.8) if shape else None
+        if case["post"]:
+            state["post_weight"] = normal(d, scale=0.1, mean=1.0)
+            state["post_bias"] = normal(d, scale=0.1) if case["bias"] else None
+        if case["train"]:
+            state["dh"] = normal(b, t, d, dtype=case["block"], scale=0.01)
+            state["ds"] = normal(b, t, d, dtype=case["stream"], scale=0.01)
+        return state
+    places, total = _places(case)
+    flat = torch.zeros(total, dtype=_TYPES[case["grads"]], device="cuda")
+    noise = normal(total, scale=0.01)
+    torch._foreach_copy_(_views(case, flat), _views(case, noise))
+    del noise
+    count = sum(n for _, n in places)
+    state = dict(case=case, flat=flat, grads=_views(case, flat), bound=case["bound"] * 0.01 * math.sqrt(count))
+    if case["op"] == "step":
+        state["weights"] = normal(total, scale=0.05)
+        state["momentum"] = torch.zeros(total, device="cuda")
+        state["optimizer"] = None
+    return state
+
+
+def _embed(state):
+    case, ids, weight = state["case"], state["ids"], state["weight"]
+    pad = 0 if case["pad"] else None
+    if own:
+        from grace_amd.ops.embedding import embedding
+
+        if not case["train"]:
+            return embedding(ids, weight, scale=case["scale"], padding_idx=pad, dtype=_TYPES[case["out"]])
+        weight.requires_grad_()
+        y = embedding(ids, weight, scale=case["scale"], padding_idx=pad, dtype=_TYPES[case["out"]])
+        return y.detach(), torch.autograd.grad(y, weight, state["dy"])[0]
+    y = (weight[ids].float() * case["scale"]).to(_TYPES[case["out"]])
+    if not case["train"]:
+        return y
+    dw = torch.zeros(weight.shape, device="cuda")
+    dw.index_add_(0, ids.reshape(-1), state["dy"].reshape(-1, weight.shape[1]).float() * case["scale"])
+    if pad is not None:
+        dw[pad] = 0
+    return y, dw.to(weight.dtype)
+
+
+def _hat(v, kind):
+    """(normalised rows, 1 / deviation)"""
+    if kind == "layer":
+        v = v - v.mean(-1, keepdim=True)
+    rstd = (v * v).mean(-1, keepdim=True).add(1e-5).rsqrt()
+    return v * rstd, rstd
+
+
+def _hat_back(hat, rstd, a, kind):
+    """The gradient through _hat for the gradient a of the normalised rows."""
+    a = a - hat * (a * hat).mean(-1, keepdim=True)
+    if kind == "layer":
+        a = a - a.mean(-1, keepdim=True)  # the mean of hat is zero
+    return a * rstd
+
+
+def _affine(hat, weight, bias):
+    return hat * weight if bias is None else hat * weight + bias
+
+
+def _norm(state):
+    case = state["case"]
+    x, y, weight, bias, gate = state["x"], state["y"], state["weight"], state["bias"], state["gate"]
+    post_weight, post_bias = state.get("post_weight"), state.get("post_bias")
+    if own:
+        from grace_amd.ops.norm import residual_norm
+
+        leaves = {"dx": x, "dy": y, "dgate": gate, "dweight": weight, "dbias": bias, "dpost_weight": post_weight,
+                  "dpost_bias": post_bias}
+        leaves = {k: v for k, v in leaves.items() if v is not None}
+        if case["train"]:
+            [v.requires_grad_() for v in leaves.values()]
+        h, s = residual_norm(y, x, weight, bias, kind=case["kind"], eps=1e-5, gate=gate, alpha=case["alpha"],
+                             post=case["post"], post_weight=post_weight, post_bias=post_bias, return_sum=True)
+        if not case["train"]:
+            return {"h": h, "s": s}
+        grads = torch.autograd.grad([h, s], list(leaves.values()), [state["dh"], state["ds"]])
+        return {"h": h.detach(), "s": s.detach(), **dict(zip(leaves, grads))}
+    kind, alpha = case["kind"], case["alpha"]
+    u = y.float()
+    if case["post"]:
+        post_hat, post_rstd = _hat(u, kind)
+        u = _affine(post_hat, post_weight, post_bias)
+    s = alpha * x.float() + (u if gate is None else gate.float() * u)
+    hat, rstd = _hat(s, kind)
+    out = {"h": _affine(hat, weight, bias).to(y.dtype), "s": s.to(x.dtype)}
+    if not case["train"]:
+        return out
+    dh = state["dh"].float()
+    ds = _hat_back(hat, rstd, dh * weight, kind) + state["ds"].float()
+    out["dx"] = (alpha * ds).to(x.dtype)
+    out["dweight"] = (dh * hat).sum((0, 1))
+    if bias is not None:
+        out["dbias"] = dh.sum((0, 1))
+    du = ds
+    if gate is not None:
+        du = gate.float() * ds
+        dgate = ds * u
+        out["dgate"] = {"channel": lambda: dgate.sum((0, 1)), "sample": lambda: dgate.sum(1, keepdim=True),
+                        "full": lambda: dgate}[case["gate"]]().to(gate.dtype)
+    if case["post"]:
+        out["dpost_weight"] = (du * post_hat).sum((0, 1))
+        if post_bias is not None:
+            out["dpost_bias"] = du.sum((0, 1))
+        du = _hat_back(post_hat, post_rstd, du * post_weight, kind)
+    out["dy"] = du.to(y.dtype)
+    return out
+
+
+def _norm_and_factor(grads, bound):
+    norm = torch.stack(torch._foreach_norm(grads, 2.0, dtype=torch.float32)).square().sum().sqrt()
+    return norm, (bound / (norm + 1e-6)).clamp(max=1.0)
+
+
+def _clip(state):
+    grads = state["grads"]
+    if own:
+        from grace_amd.parallel import clip_grad_norm_
+
+        norm = clip_grad_norm_(grads, state["bound"])
+    else:
+        norm, factor = _norm_and_factor(grads, state["bound"])
+        wide = grads if grads[0].dtype == torch.float32 else [g.float() for g in grads]
+        torch._foreach_copy_(grads, torch._foreach_mul(wide, factor))
+    return {"grads": state["flat"], "norm": norm}
+
+
+def _step(state):
+    grads = state["grads"]
+    if own:
+        from grace_amd.parallel import FusedSGD
+
+        opt = state["optimizer"]
+        if opt is None:
+            params = [torch.nn.Parameter(w) for w in _views(state["case"], state["weights"])]
+            [setattr(p, "grad", g) for p, g in zip(params, grads)]
+            opt = state["optimizer"] = FusedSGD(params, lr=_LR, momentum=_MOMENTUM, weight_decay=_DECAY,
+                                                max_grad_norm=state["bound"])
+        opt.step()
+        return {"weights": state["weights"], "norm": opt.grad_norm}
+    if state["optimizer"] is None:
+        state["optimizer"] = _views(state["case"], state["weights"]), _views(state["case"], state["momentum"])
+    weights, momentum = state["optimizer"]
+    norm, factor = _norm_and_factor(grads, state["bound"])
+    scaled = torch._foreach_mul(grads, factor)
+    torch._foreach_add_(scaled, weights, alpha=_DECAY)
+    torch._foreach_mul_(momentum, _MOMENTUM)
+    torch._foreach_add_(momentum, scaled)
+    torch._foreach_add_(weights, momentum, alpha=-_LR)
+    return {"weights": state["weights"], "norm": norm}
+
+
+def run(state):
+    return {"embed": _embed, "norm": _norm, "clip": _clip, "step": _step}[state["case"]["op"]](state)
+
+
+def work(case):
+    if case["op"] == "embed":
+        n, d, v = case["batch"] * case["length"], case["width"], case["vocab"]
+        table, out = _BYTES[case["table"]], _BYTES[case["out"]]
+        rows = min(n, v)  # at most so many rows are read
+        moved, flops = n * _BYTES[case["index"]] + rows * d * table + n * d * out, n * d
+        if case["train"]:
+            moved += n * d * out + v * d * table
+            flops += n * d
+        return {"bytes": moved, "flops": flops}
+    if case["op"] == "norm":
+        n = case["batch"] * case["length"] * case["width"]
+        stream, block = _BYTES[case["stream"]], _BYTES[case["block"]]
+        gate = {"none": 0, "channel": case["width"], "sample": case["batch"] * case["width"], "full": n}[case["gate"]]
+        gate *= block
+        moved, flops = n * 2 * (stream + block) + gate, n * (8 + (8 if case["post"] else 0))
+        if case["train"]:
+            uses_y = case["post"] or case["gate"] != "none"
+            one = not uses_y and case["alpha"] == 1.0 and stream == block  # dx and dy are one and the same
+            moved += n * (3 * stream + block + (0 if one else block) + (block if uses_y else 0)) + 2 * gate
+            flops += n * (14 + (14 if case["post"] else 0))
+        return {"bytes": moved, "flops": flops}
+    n, size = sum(_sizes(case)), _BYTES[case["grads"]]
+    if case["op"] == "clip":  # under the bound the gradients are only read
+        return {"bytes": n * size * (1 if case["bound"] > 1 else 2), "flops": 2 * n}
+    return {"bytes": n * 4 * 5, "flops": 8 * n}
+
+
+def exact(case, seed):
+    state = prepare(case, seed)
+    if case["op"] == "embed":
+        ids, weight = state["ids"].reshape(-1).long(), state["weight"].double()
+        y = torch.index_select(weight, 0, ids).mul_(case["scale"]).view(case["batch"], case["length"], -1)
+        if not case["train"]:
+            return y
+        dy = state["dy"].double().reshape(ids.numel(), -1)
+        if case["pad"]:
+            dy[ids == 0] = 0
+        order = torch.argsort(ids, stable=True)
+        found, counts = torch.unique_consecutive(ids[order], return_counts=True)
+        sums = torch.segment_reduce(dy[order], "sum", lengths=counts, axis=0)
+        dw = torch.zeros_like(weight)
+        dw[found] = sums * case["scale"]
+        return y, dw
+    if case["op"] == "norm":
+        names = ["x", "y", "gate", "weight", "bias", "post_weight", "post_bias"]
+        v = {k: state[k].double().requires_grad_(case["train"]) for k in names if state.get(k) is not None}
+
+        def rows(z, w, b):
+            centre = z.mean(-1, keepdim=True) if case["kind"] == "layer" else 0.0
+            z = (z - centre) / torch.sqrt(((z - centre) ** 2).mean(-1, keepdim=True) + 1e-5)
+            z = z * w
+            return z if b is None else z + b
+
+        with torch.set_grad_enabled(case["train"]):
+            u = rows(v["y"], v["post_weight"], v.get("post_bias")) if case["post"] else v["y"]
+            s = case["alpha"] * v["x"] + (u * v["gate"] if "gate" in v else u)
+            h = rows(s, v["weight"], v.get("bias"))
+        out = {"h": h.detach(), "s": s.detach()}
+        if case["train"]:
+            got = torch.autograd.grad([h, s], list(v.values()), [state["dh"].double(), state["ds"].double()])
+            out.update({"d" + k: g for k, g in zip(v, got)})
+        return out
+    grads = state["flat"].double()
+    norm = torch.linalg.vector_norm(grads)
+    factor = min(1.0, state["bound"] / (norm.item() + 1e-6))
+    if case["op"] == "clip":
+        return {"grads": grads * factor, "norm": norm}
+    used = torch.zeros_like(grads, dtype=torch.bool)
+    for at, n in _places(case)[0]:
+        used[at:at + n] = True
+    weights = state["weights"].double()
+    moved = weights - _LR * (grads * factor + _DECAY * weights)
+    return {"weights": torch.where(used, moved, weights), "norm": norm}
