@@ -156,12 +156,15 @@ def prepare(case, seed):
     places, total = _places(case)
     flat = torch.zeros(total, dtype=_TYPES[case["grads"]], device="cuda")
     noise = normal(total, scale=0.01)
-    torch._foreach_copy_(_views(case, flat), _views(case, noise))
+    torch._foreach_copy_(_views(case, flat), _views(case, noise))  # zeros between the tensors
     del noise
     count = sum(n for _, n in places)
-    state = dict(case=case, flat=flat, grads=_views(case, flat), bound=case["bound"] * 0.01 * math.sqrt(count))
+    state = dict(case=case, flat=flat, grads=_views(case, flat), bound=case["bound"] * 0.01 * math.sqrt(count),
+                 weights=normal(total, dtype=case["grads"], scale=0.05))
+    state["params"] = [torch.nn.Parameter(w) for w in _views(case, state["weights"])]
+    for p, g in zip(state["params"], state["grads"]):
+        p.grad = g
     if case["op"] == "step":
-        state["weights"] = normal(total, scale=0.05)
         state["momentum"] = torch.zeros(total, device="cuda")
         state["optimizer"] = None
     return state
@@ -267,7 +270,7 @@ def _clip(state):
     if own:
         from grace_amd.parallel import clip_grad_norm_
 
-        norm = clip_grad_norm_(grads, state["bound"])
+        norm = clip_grad_norm_(state["params"], state["bound"])
     else:
         norm, factor = _norm_and_factor(grads, state["bound"])
         wide = grads if grads[0].dtype == torch.float32 else [g.float() for g in grads]
@@ -282,9 +285,7 @@ def _step(state):
 
         opt = state["optimizer"]
         if opt is None:
-            params = [torch.nn.Parameter(w) for w in _views(state["case"], state["weights"])]
-            [setattr(p, "grad", g) for p, g in zip(params, grads)]
-            opt = state["optimizer"] = FusedSGD(params, lr=_LR, momentum=_MOMENTUM, weight_decay=_DECAY,
+            opt = state["optimizer"] = FusedSGD(state["params"], lr=_LR, momentum=_MOMENTUM, weight_decay=_DECAY,
                                                 max_grad_norm=state["bound"])
         opt.step()
         return {"weights": state["weights"], "norm": opt.grad_norm}
