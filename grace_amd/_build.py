@@ -72,6 +72,8 @@ def _common_flags(inc_dirs, abi):
         "-std=c++17",
         "-fPIC",
         "-munsafe-fp-atomics",
+        # no packed fp32 instructions: some of their forms have given wrong results on gfx950
+        "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
         f"-D_GLIBCXX_USE_CXX11_ABI={abi}",
         "-DTORCH_EXTENSION_NAME=_C",
         "-DTORCH_API_INCLUDE_EXTENSION_H",
