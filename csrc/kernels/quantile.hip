@@ -61,6 +61,14 @@ __device__ __forceinline__ float key_value(uint32_t k) {
   return __uint_as_float((k & 0x80000000u) ? (k & 0x7fffffffu) : ~k);
 }
 
+// torch's a * (1 - w) + b * w: every step rounded by itself.  __fmul_rn and __fadd_rn are plain
+// operators in HIP's headers, which the compiler may contract to an fma; the pragma forbids that.
+__device__ __forceinline__ float interpolate(float a, float b, float w) {
+#pragma clang fp contract(off)
+  const float p = a * (1.f - w), q = b * w;
+  return p + q;
+}
+
 // first index >= b whose address is 16-B aligned (clamped to e): scalar head, float4 body
 __device__ __forceinline__ int64_t aligned_begin(const float* x, int64_t b, int64_t e) {
   const int64_t mis = (int64_t)((reinterpret_cast<uintptr_t>(x) >> 2) & 3);
@@ -306,8 +314,7 @@ __global__ __launch_bounds__(kSelBlock) void qsel_select_kernel(
     const int64_t eb = (int64_t)seg * (q + 1);
     for (int j = t; j <= q; j += kSelBlock) {
       const float a = vals[lo_idx[eb + j]], bv = vals[hi_idx[eb + j]], ww = w[eb + j];
-      // torch: a * (1 - w) + b * w, three separately rounded ops
-      edges[eb + j] = __fadd_rn(__fmul_rn(a, __fsub_rn(1.f, ww)), __fmul_rn(bv, ww));
+      edges[eb + j] = interpolate(a, bv, ww);
     }
   }
 }
