@@ -1075,6 +1075,7 @@ std::string build_info() {
 
 void grace_bind_comm(py::module& m);  // csrc/comm/rccl_comm.cpp
 void grace_bind_nn(py::module& m);    // csrc/nn_bindings.cpp
+void grace_bind_lm(py::module& m);    // csrc/lm_bindings.cpp
 void grace_bind_xgmi(py::module& m);  // csrc/comm/xgmi_allgather.hip
 void grace_bind_health(py::module& m);  // csrc/comm/health.cpp
 void grace_bind_runtime(py::module& m);  // csrc/runtime/graph_split.cpp
@@ -1223,6 +1224,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   grace_bind_runtime(m);
   grace_bind_comm(m);
   grace_bind_nn(m);
+  grace_bind_lm(m);
   grace_bind_xgmi(m);
   grace_bind_health(m);
   m.doc() = "grace_amd native CDNA4 kernels and RCCL runtime";

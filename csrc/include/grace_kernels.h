@@ -329,8 +329,9 @@ void health_init(int device = -1);
 // it is safe while a stream is being captured)
 uint32_t* health_dev(int device);
 
+// clip: a device factor that every gradient is multiplied by first, or nullptr
 void sgd_step(float* const* p, const float* const* g, float* const* buf, uint16_t* const* w16, const int64_t* len,
               int n_seg, float lr, float momentum, float dampening, float wd, bool nesterov, bool maximize,
-              bool first, hipStream_t stream);
+              bool first, const float* clip, hipStream_t stream);
 
 }  // namespace grace

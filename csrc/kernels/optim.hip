@@ -5,6 +5,7 @@
 // tensor i owns blocks [start[i], start[i+1]) and a block finds its tensor by binary search, so
 // small tensors cost one block, not a strided grid row.  float4 accesses.  Per element
 // (maximize flips g first):
+//     g   = clip * g                                                  (clip: a device value, optional)
 //     g   = g + wd * p
 //     buf = first ? g : momentum * buf + (1 - dampening) * g         (momentum != 0)
 //     g   = nesterov ? g + momentum * buf : buf
@@ -40,7 +41,8 @@ struct SgdHyper {
   int nesterov, maximize, first;
 };
 
-__device__ __forceinline__ float sgd_elem(float& p, float g, float* bufp, const SgdHyper& h) {
+__device__ __forceinline__ float sgd_elem(float& p, float g, float* bufp, const SgdHyper& h, float clip) {
+  if (clip != 1.f) g *= clip;
   if (h.maximize) g = -g;
   if (h.wd != 0.f) g = fmaf(h.wd, p, g);
   if (bufp) {
@@ -52,8 +54,10 @@ __device__ __forceinline__ float sgd_elem(float& p, float g, float* bufp, const 
   return p;
 }
 
-__global__ __launch_bounds__(kBlock) void sgd_kernel(SgdTable t, SgdHyper h, const uint32_t* __restrict__ fault) {
+__global__ __launch_bounds__(kBlock) void sgd_kernel(SgdTable t, SgdHyper h, const uint32_t* __restrict__ fault,
+                                                     const float* __restrict__ clip_factor) {
   if (fault != nullptr && __hip_atomic_load(fault, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) != 0u) return;
+  const float clip = clip_factor != nullptr ? *clip_factor : 1.f;
   int lo = 0, hi = t.n - 1;  // last tensor with start <= blockIdx.x
   while (lo < hi) {
     const int mid = (lo + hi + 1) >> 1;
@@ -93,10 +97,10 @@ __global__ __launch_bounds__(kBlock) void sgd_kernel(SgdTable t, SgdHyper h, con
     for (int u = 0; u < U; ++u) {
       const int64_t i = threadIdx.x + (int64_t)u * stride;
       if (i >= nv) continue;
-      sgd_elem(pv[u].x, gv[u].x, m ? &bv[u].x : nullptr, h);
-      sgd_elem(pv[u].y, gv[u].y, m ? &bv[u].y : nullptr, h);
-      sgd_elem(pv[u].z, gv[u].z, m ? &bv[u].z : nullptr, h);
-      sgd_elem(pv[u].w, gv[u].w, m ? &bv[u].w : nullptr, h);
+      sgd_elem(pv[u].x, gv[u].x, m ? &bv[u].x : nullptr, h, clip);
+      sgd_elem(pv[u].y, gv[u].y, m ? &bv[u].y : nullptr, h, clip);
+      sgd_elem(pv[u].z, gv[u].z, m ? &bv[u].z : nullptr, h, clip);
+      sgd_elem(pv[u].w, gv[u].w, m ? &bv[u].w : nullptr, h, clip);
       reinterpret_cast<float4*>(p)[i] = pv[u];
       if (m) reinterpret_cast<float4*>(buf)[i] = bv[u];
       if (w) {
@@ -110,7 +114,7 @@ __global__ __launch_bounds__(kBlock) void sgd_kernel(SgdTable t, SgdHyper h, con
   }
   for (int64_t i = tail + threadIdx.x; i < n; i += stride) {
     float pv = p[i];
-    sgd_elem(pv, g[i], buf ? buf + i : nullptr, h);
+    sgd_elem(pv, g[i], buf ? buf + i : nullptr, h, clip);
     p[i] = pv;
     if (w) w[i] = f32_to_bf16_rne(pv);
   }
@@ -120,7 +124,7 @@ __global__ __launch_bounds__(kBlock) void sgd_kernel(SgdTable t, SgdHyper h, con
 
 void sgd_step(float* const* p, const float* const* g, float* const* buf, uint16_t* const* w16, const int64_t* len,
               int n_seg, float lr, float momentum, float dampening, float wd, bool nesterov, bool maximize,
-              bool first, hipStream_t stream) {
+              bool first, const float* clip, hipStream_t stream) {
   // the fault word of the device this stream launches on (never another GPU's memory)
   int dev = -1;
   if (hipStreamGetDevice(stream, &dev) != hipSuccess) {
@@ -145,7 +149,7 @@ void sgd_step(float* const* p, const float* const* g, float* const* buf, uint16_
     t.start[m] = nb;
     t.n = m;
     const uint32_t* fault = dev_fault ? dev_fault + kHealthFault : nullptr;
-    if (nb > 0) hipLaunchKernelGGL(sgd_kernel, dim3((unsigned)nb), dim3(kBlock), 0, stream, t, h, fault);
+    if (nb > 0) hipLaunchKernelGGL(sgd_kernel, dim3((unsigned)nb), dim3(kBlock), 0, stream, t, h, fault, clip);
   }
 }
 

@@ -1,0 +1,156 @@
+// Launchers of the residual norms (the kernels, and the mathematics: grace_resnorm.h).
+#include "grace_resnorm.h"
+
+namespace grace {
+
+namespace resnorm {
+GRACE_RESNORM_DECLARE(extern, float, float)
+GRACE_RESNORM_DECLARE(extern, bf16_t, bf16_t)
+GRACE_RESNORM_DECLARE(extern, float, bf16_t)
+GRACE_RESNORM_DECLARE(extern, half_t, half_t)
+GRACE_RESNORM_DECLARE(extern, float, half_t)
+}  // namespace resnorm
+
+namespace {
+
+using namespace resnorm;
+
+constexpr int kMaxParts = 1024;  // partial rows of the column sums
+constexpr int kMinRows = 4;      // rows per row slot of a workgroup before another workgroup is added
+
+struct FoldArgs {
+  const float* part;
+  int64_t blocks;
+  int d;
+  int sums;            // outputs below: the wanted sums in turn
+  int which[kSums];
+  void* out[kSums];
+  bool f32[kSums];
+  int64_t rows[kSums];  // output rows (more than one: dgate's groups)
+};
+
+// One workgroup adds 64 columns of one output row: 16 waves take every 16th partial row each.
+template <typename TY>
+__global__ __launch_bounds__(1024) void resnorm_fold_kernel(FoldArgs a) {
+  int64_t row = blockIdx.y;
+  int k = 0;
+  while (k + 1 < a.sums && row >= a.rows[k]) row -= a.rows[k++];
+  const int64_t per = a.blocks / a.rows[k];
+  const int c = blockIdx.x * kWave + lane_id();
+  float v = 0.f;
+  if (c < a.d) {
+    const float* p = a.part + ((int64_t)a.which[k] * a.blocks + row * per) * a.d + c;
+    for (int64_t i = wave_id(); i < per; i += 16) v += p[i * a.d];
+  }
+  __shared__ float red[16][kWave];
+  red[wave_id()][lane_id()] = v;
+  __syncthreads();
+  if (wave_id() == 0 && c < a.d) {
+    for (int i = 1; i < 16; ++i) v += red[i][lane_id()];
+    const float o[1] = {v};
+    store_param<TY>(a.out[k], a.f32[k], row * a.d + c, o, 1);
+  }
+}
+
+int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// row slots of a workgroup
+int row_slots(int d, bool full) {
+  int slots = 1;
+  by_width(d, full, [&](auto, auto tpr) { slots = block_of<decltype(tpr)::value>() / decltype(tpr)::value; });
+  return slots;
+}
+
+Split split_rows(const NormShape& n, bool full, bool grouped) {
+  const int slots = row_slots(n.d, full);
+  const int64_t most = std::max<int64_t>(1, std::min<int64_t>(kMaxParts, cdiv(n.rows, (int64_t)slots * kMinRows)));
+  Split s{1, n.rows, most, 1, most};
+  if (grouped && n.gate_rows < n.rows) {
+    s.groups = n.rows / n.gate_rows;
+    s.group_rows = n.gate_rows;
+    s.parts = std::max<int64_t>(1, most / s.groups);
+    s.per_block = s.parts > 1 ? 1 : cdiv(s.groups, most);
+    s.blocks = s.parts > 1 ? s.groups * s.parts : cdiv(s.groups, s.per_block);
+  }
+  return s;
+}
+
+template <typename F>
+void by_types(const NormShape& n, F&& f) {
+  using std::integral_constant;
+  if (n.ty == ElType::kF32) return f((float*)nullptr, (float*)nullptr);
+  if (n.ty == ElType::kBF16)
+    return n.tx == ElType::kF32 ? f((float*)nullptr, (bf16_t*)nullptr) : f((bf16_t*)nullptr, (bf16_t*)nullptr);
+  return n.tx == ElType::kF32 ? f((float*)nullptr, (half_t*)nullptr) : f((half_t*)nullptr, (half_t*)nullptr);
+}
+
+}  // namespace
+
+void resnorm_forward(const NormShape& n, const void* x, const void* y, NormParam gate, NormParam weight, NormParam bias,
+                     NormParam post_weight, NormParam post_bias, void* h, void* s, float* stats, hipStream_t stream) {
+  if (n.rows == 0 || n.d == 0) return;
+  const FwdArgs a{n, x, y, gate, weight, bias, post_weight, post_bias, h, s, stats};
+  by_types(n, [&](auto* tag_x, auto* tag_y) {
+    using TX = std::remove_pointer_t<decltype(tag_x)>;
+    using TY = std::remove_pointer_t<decltype(tag_y)>;
+    launch_forward<TX, TY>(a, stream);
+  });
+}
+
+int64_t resnorm_backward_ws(const NormShape& n) {
+  int64_t blocks = 1;
+  for (bool full : {false, true})
+    for (bool grouped : {false, true}) blocks = std::max(blocks, split_rows(n, full, grouped).blocks);
+  return kSums * blocks * n.d * (int64_t)sizeof(float);
+}
+
+void resnorm_backward(const NormShape& n, const void* s, const void* y, const float* stats, NormParam gate,
+                      NormParam weight, NormParam post_weight, NormParam post_bias, const void* dh, const void* ds,
+                      const NormGrads& g, void* ws, hipStream_t stream) {
+  if (n.rows == 0 || n.d == 0) return;
+  const bool full = gate.p != nullptr || n.post;
+  const bool own_rows = n.gate_rows == 1 && n.rows > 1;  // the gate has the rows' own shape
+  BwdArgs a{};
+  a.n = n;
+  a.split = split_rows(n, full, g.dgate != nullptr && !own_rows);
+  a.s = s;
+  a.y = y;
+  a.dh = dh;
+  a.ds = ds;
+  a.stats = stats;
+  a.gate = gate;
+  a.weight = weight;
+  a.post_weight = post_weight;
+  a.post_bias = post_bias;
+  a.dx = g.dx == g.dy ? nullptr : g.dx;
+  a.dy = g.dy;
+  a.dgate = g.dgate;
+  a.dgate_f32 = gate.f32;
+  a.dgate_mode = g.dgate == nullptr ? 0 : own_rows ? 3 : a.split.groups > 1 && a.split.parts == 1 ? 2 : 1;
+  a.part = static_cast<float*>(ws);
+  void* const outs[kSums] = {g.dweight, g.dbias, a.dgate_mode == 1 ? g.dgate : nullptr, g.dpost_weight, g.dpost_bias};
+  FoldArgs f{};
+  f.part = a.part;
+  f.blocks = a.split.blocks;
+  f.d = n.d;
+  const bool f32[kSums] = {weight.f32, g.bias_f32, gate.f32, post_weight.f32, g.post_bias_f32};
+  int64_t out_rows = 0;
+  for (int k = 0; k < kSums; ++k) {
+    a.want[k] = outs[k] != nullptr;
+    if (!outs[k]) continue;
+    f.which[f.sums] = k;
+    f.out[f.sums] = outs[k];
+    f.f32[f.sums] = f32[k];
+    f.rows[f.sums] = k == kDg ? a.split.groups : 1;
+    out_rows += f.rows[f.sums++];
+  }
+  by_types(n, [&](auto* tag_x, auto* tag_y) {
+    using TX = std::remove_pointer_t<decltype(tag_x)>;
+    using TY = std::remove_pointer_t<decltype(tag_y)>;
+    launch_backward<TX, TY>(a, full, stream);
+    if (f.sums > 0)
+      resnorm_fold_kernel<TY><<<dim3((unsigned)cdiv(n.d, kWave), (unsigned)out_rows), 1024, 0, stream>>>(f);
+  });
+}
+
+}  // namespace grace

@@ -251,7 +251,8 @@ std::vector<Tensor> bn_act_bwd_partials(const Tensor& dy, const Tensor& x, const
 // with the parameter's strides).  bufs / w16 entries may be None.
 void sgd_step(const std::vector<Tensor>& params, const std::vector<Tensor>& grads,
               const std::vector<c10::optional<Tensor>>& bufs, const std::vector<c10::optional<Tensor>>& w16,
-              double lr, double momentum, double dampening, double wd, bool nesterov, bool maximize, bool first) {
+              double lr, double momentum, double dampening, double wd, bool nesterov, bool maximize, bool first,
+              const c10::optional<Tensor>& clip) {
   const size_t n = params.size();
   TORCH_CHECK(grads.size() == n && bufs.size() == n && w16.size() == n, "sgd_step: list lengths");
   if (n == 0) return;
@@ -285,9 +286,15 @@ void sgd_step(const std::vector<Tensor>& params, const std::vector<Tensor>& grad
     }
     len[i] = t.numel();
   }
+  const float* factor = nullptr;
+  if (clip.has_value() && clip->defined()) {
+    TORCH_CHECK(clip->device() == params[0].device() && clip->scalar_type() == at::kFloat && clip->numel() == 1,
+                "sgd_step: the clip factor must be one fp32 value on the parameters' device");
+    factor = clip->data_ptr<float>();
+  }
   DevGuard guard(params[0].device());
   grace::sgd_step(p.data(), g.data(), b.data(), w.data(), len.data(), (int)n, (float)lr, (float)momentum,
-                  (float)dampening, (float)wd, nesterov, maximize, first, cur_stream());
+                  (float)dampening, (float)wd, nesterov, maximize, first, factor, cur_stream());
 }
 // conv bias (+ ReLU): y = act(x + bias) for channels_last [N, C, H, W] x
 Tensor bias_act_fwd(const Tensor& x, const Tensor& bias, bool relu) {
@@ -411,7 +418,9 @@ void grace_bind_nn(py::module& m) {
         py::arg("s"), py::arg("pad"), py::arg("dy2") = py::none());
   m.def("bias_act_fwd", &bias_act_fwd);
   m.def("bias_act_bwd", &bias_act_bwd);
-  m.def("sgd_step", &sgd_step);
+  m.def("sgd_step", &sgd_step, py::arg("params"), py::arg("grads"), py::arg("bufs"), py::arg("w16"), py::arg("lr"),
+        py::arg("momentum"), py::arg("dampening"), py::arg("wd"), py::arg("nesterov"), py::arg("maximize"),
+        py::arg("first"), py::arg("clip") = py::none());
   m.def("bn_supported", &bn_supported);
   m.def("bn_fused_v", [](int64_t M, int64_t C, bool bwd) { return grace::bn_fused_v(M, (int)C, bwd); });
   m.def("bn_set_fused", &grace::bn_set_fused);

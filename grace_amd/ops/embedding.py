@@ -1,0 +1,92 @@
+"""Embedding lookup with scaling, and its gradient by sorted tokens (``csrc/kernels/embed.hip``).
+
+``embedding(ids, weight, scale)`` is ``round(scale * weight[ids])``; its gradient sums the rows of the
+output's gradient over equal tokens in fp32 (fp64 for an fp64 table on the CPU), in token order, and
+rounds once to the table's type.  On a GPU the tokens are sorted by row and runs of equal tokens are
+summed in a fixed order: no atomics, the same result on every call.  Every row of the gradient is written,
+untouched rows as zeros.
+
+A token outside the table raises ``IndexError`` on the CPU.  On a GPU, where that check would
+need a device synchronisation, its output row is NaN and it adds nothing to the gradient.
+"""
+from __future__ import annotations
+
+from typing import Optional
+
+import torch
+import torch.nn as nn
+import torch.nn.functional as F
+from torch.autograd.function import once_differentiable
+
+from . import _native
+
+_DTYPES = (torch.float32, torch.bfloat16, torch.float16)
+
+
+class _EmbeddingFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, weight, ids, scale, pad, dtype):
+        ctx.save_for_backward(ids)
+        ctx.args = (weight.shape[0], pad, scale, weight.dtype)
+        return _native.lib().embed_fwd(ids, weight, scale, dtype)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        (ids,) = ctx.saved_tensors
+        vocab, pad, scale, dtype = ctx.args
+        return _native.lib().embed_bwd(ids, dy.contiguous(), vocab, pad, scale, dtype), None, None, None, None
+
+
+def embedding(ids: torch.Tensor, weight: torch.Tensor, scale: float = 1.0, padding_idx: Optional[int] = None,
+              dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+    """``round(scale * weight[ids])`` of shape ``[*ids.shape, width]``.
+
+    ``ids``: int64 or int32, any shape and strides.  ``weight``: ``[rows, width]``, float32, bfloat16 or
+    float16.  ``dtype``: the output's type (default: the table's).  ``padding_idx`` (negative: from the end)
+    names a row that gets no gradient.  Differentiable once, in ``weight``."""
+    if ids.dtype not in (torch.int64, torch.int32):
+        raise TypeError(f"embedding: ids must be int64 or int32, got {ids.dtype}")
+    if weight.dim() != 2:
+        raise ValueError(f"embedding: the table must be [rows, width], got {tuple(weight.shape)}")
+    if ids.device != weight.device:
+        raise ValueError(f"embedding: ids on {ids.device}, table on {weight.device}")
+    rows = weight.shape[0]
+    if rows == 0 and ids.numel() > 0:
+        raise ValueError("embedding: the table has no rows")
+    pad = -1
+    if padding_idx is not None:
+        pad = padding_idx + rows if padding_idx < 0 else padding_idx
+        if not 0 <= pad < rows:
+            raise ValueError(f"embedding: padding_idx {padding_idx} outside a table of {rows} rows")
+    dtype = weight.dtype if dtype is None else dtype
+    if _native.use_native(weight):
+        if weight.dtype not in _DTYPES or dtype not in _DTYPES:
+            raise TypeError(f"embedding: float32, bfloat16 or float16 on a GPU, got {weight.dtype} -> {dtype}")
+        if ids.numel() >= 2**31 - 1 or rows >= 2**31 - 1:
+            raise ValueError("embedding: at most 2^31 - 2 tokens and rows")
+        ids = ids.contiguous()
+        if weight.stride(1) != 1 and weight.shape[1] > 1:
+            weight = weight.contiguous()
+        if torch.is_grad_enabled() and weight.requires_grad:
+            return _EmbeddingFn.apply(weight, ids, float(scale), pad, dtype)
+        return _native.lib().embed_fwd(ids, weight, float(scale), dtype)
+    wide = weight if weight.dtype == torch.float64 else weight.float()
+    return (F.embedding(ids, wide, None if pad < 0 else pad) * float(scale)).to(dtype)
+
+
+class ScaledEmbedding(nn.Embedding):
+    """Drop-in ``nn.Embedding`` (same parameter, same state dict) on the native kernels, with a factor
+    on the looked-up rows.  ``max_norm``, ``scale_grad_by_freq`` and ``sparse`` are refused."""
+
+    def __init__(self, *args, scale: float = 1.0, **kw):
+        super().__init__(*args, **kw)
+        if self.max_norm is not None or self.scale_grad_by_freq or self.sparse:
+            raise ValueError("ScaledEmbedding: max_norm, scale_grad_by_freq and sparse are not supported")
+        self.scale = float(scale)
+
+    def forward(self, ids: torch.Tensor) -> torch.Tensor:
+        return embedding(ids, self.weight, self.scale, self.padding_idx)
+
+    def extra_repr(self) -> str:
+        return super().extra_repr() + f", scale={self.scale:g}"

@@ -1,0 +1,182 @@
+"""Norms around a block, fused with its gate and the scaled residual (``csrc/include/grace_resnorm.h``).
+
+``residual_norm(y, x, weight, bias, gate=g, alpha=a, post=True, ...)`` computes, in one pass over rows
+of the last dimension,
+
+    u = post ? N(y; post_weight, post_bias) : y      the norm after the block
+    s = a * x + g * u                                the residual stream
+    h = N(s; weight, bias)                           the norm before the next block
+
+with N a layer norm or a root-mean-square norm.  Without options it is a plain norm of ``y``; with a
+residual alone it is the post-norm step ``N(x + f(x))`` of the encoder.  Everything is computed in fp32
+(fp64 for fp64 inputs on the CPU) from the unrounded sum; ``h`` has the type of ``y``, ``s`` that of ``x``.
+The backward is one pass too: it reads ``s`` (and ``y`` where a gate or a post norm needs it), and the
+gradients of weights, biases and shared gates are summed in a fixed order.
+"""
+from __future__ import annotations
+
+from typing import Optional
+
+import torch
+import torch.nn as nn
+from torch.autograd.function import once_differentiable
+
+from . import _native
+
+_DTYPES = (torch.float32, torch.bfloat16, torch.float16)
+
+
+class _ResidualNormFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, y, x, gate, weight, bias, post_weight, post_bias, args, return_sum):
+        gate_rows, post, rms, alpha, eps = args
+        plain = x is None and gate is None and not post
+        h, s, stats = _native.lib().resnorm_fwd(y, x, gate, gate_rows, weight, bias, post_weight, post_bias, post,
+                                                rms, alpha, eps, not plain, True)
+        uses_y = gate is not None or post
+        ctx.save_for_backward(y if plain else s, y if uses_y else None, stats, gate, weight, bias, post_weight,
+                              post_bias)
+        ctx.args = args
+        ctx.dtype = y.dtype
+        ctx.set_materialize_grads(False)
+        # without residual, gate and post norm the sum is the block itself, as an output of its own: its
+        # gradient then joins the norm's before the one rounding
+        return (h, y.detach() if plain else s) if return_sum else h
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dh, ds=None):
+        if dh is None and ds is None:
+            return (None,) * 9
+        s, y, stats, gate, weight, bias, post_weight, post_bias = ctx.saved_tensors
+        gate_rows, post, rms, alpha, eps = ctx.args
+        dh = None if dh is None else dh.contiguous()
+        ds = None if ds is None else ds.contiguous()
+        if y is None:  # only its type and shape count
+            y = dh if dh is not None else torch.empty(s.shape, dtype=ctx.dtype, device=s.device)
+        need = ctx.needs_input_grad
+        dx, dy, *rest = _native.lib().resnorm_bwd(dh, ds, s, y, stats, gate, gate_rows, weight, bias, post_weight,
+                                                  post_bias, post, rms, alpha, eps, [need[1], need[0], *need[2:7]])
+        return (dy if need[0] else None, dx, *rest, None, None)
+
+
+def _gate_rows(gate: torch.Tensor, y: torch.Tensor) -> int:
+    """Consecutive rows of y that share one row of the gate."""
+    lead = y.shape[:-1]
+    g = gate.shape[:-1] if gate.dim() == y.dim() else (1,) * len(lead) if gate.dim() == 1 else None
+    if g is not None and gate.shape[-1] == y.shape[-1]:
+        k = 0
+        while k < len(lead) and g[k] == lead[k]:
+            k += 1
+        if all(n == 1 for n in g[k:]):
+            rows = 1
+            for n in lead[k:]:
+                rows *= n
+            return rows
+    raise ValueError(f"residual_norm: a gate of shape {tuple(gate.shape)} for a block of {tuple(y.shape)}: it is "
+                     "[width], or the block's shape with 1 in place of trailing dimensions before the last")
+
+
+def _torch_norm(v, weight, bias, rms, eps):
+    if not rms:
+        v = v - v.mean(-1, keepdim=True)
+    v = v * torch.rsqrt(v.square().mean(-1, keepdim=True) + eps)
+    if weight is not None:
+        v = v * weight
+    return v if bias is None else v + bias
+
+
+def residual_norm(y: torch.Tensor, residual: Optional[torch.Tensor] = None, weight: Optional[torch.Tensor] = None,
+                  bias: Optional[torch.Tensor] = None, *, kind: str = "layer", eps: float = 1e-5,
+                  gate: Optional[torch.Tensor] = None, alpha: float = 1.0, post: bool = False,
+                  post_weight: Optional[torch.Tensor] = None, post_bias: Optional[torch.Tensor] = None,
+                  return_sum: bool = False):
+    """``h``, or ``(h, s)`` with ``return_sum`` (the module's docstring has the formulas).
+
+    ``y``: the block's output ``[..., width]``, float32, bfloat16 or float16, width at most 16384 on a GPU.
+    ``residual``: the stream, of y's shape, of its type or float32.  ``weight``, ``bias``, ``post_weight``,
+    ``post_bias``: ``[width]``; ``gate``: ``[width]``, or y's shape with 1 in place of trailing dimensions
+    before the last (``[batch, 1, width]``: one gate a sample); each float32 or of y's type.  ``alpha``
+    scales the residual and has no gradient.  Tensors that are not contiguous are copied first.
+    Differentiable once."""
+    if kind not in ("layer", "rms"):
+        raise ValueError(f"residual_norm: kind {kind!r}: 'layer' or 'rms'")
+    if y.dim() < 1 or y.shape[-1] < 1:
+        raise ValueError(f"residual_norm: a block of shape {tuple(y.shape)}")
+    if not post and (post_weight is not None or post_bias is not None):
+        raise ValueError("residual_norm: post_weight and post_bias need post=True")
+    native = _native.use_native(y)
+    if y.dtype not in _DTYPES and (native or y.dtype != torch.float64):
+        raise TypeError(f"residual_norm: a block of {y.dtype}")
+    width = y.shape[-1]
+    if residual is None:
+        if alpha != 1.0:
+            raise ValueError("residual_norm: alpha scales a residual, and there is none")
+    else:
+        if residual.shape != y.shape or residual.device != y.device:
+            raise ValueError(f"residual_norm: a residual of {tuple(residual.shape)} on {residual.device} for a block "
+                             f"of {tuple(y.shape)} on {y.device}")
+        if residual.dtype not in (y.dtype, torch.float32) or y.dtype == torch.float64 != residual.dtype:
+            raise TypeError(f"residual_norm: a residual of {residual.dtype} for a block of {y.dtype}")
+    for name, p in (("weight", weight), ("bias", bias), ("post_weight", post_weight), ("post_bias", post_bias),
+                    ("gate", gate)):
+        if p is None:
+            continue
+        if p.device != y.device:
+            raise ValueError(f"residual_norm: {name} on {p.device}, the block on {y.device}")
+        if p.dtype not in (y.dtype, torch.float32):
+            raise TypeError(f"residual_norm: {name} of {p.dtype} for a block of {y.dtype}")
+        if name != "gate" and p.shape != (width,):
+            raise ValueError(f"residual_norm: {name} of shape {tuple(p.shape)} for a width of {width}")
+    gate_rows = y.numel() // width
+    if gate is not None:
+        gate_rows = _gate_rows(gate, y)
+    rms, eps, alpha = kind == "rms", float(eps), float(alpha)
+    plain = residual is None and gate is None and not post
+    if not native:
+        wide = torch.float64 if y.dtype == torch.float64 else torch.float32
+        w = [None if p is None else p.to(wide) for p in (weight, bias, post_weight, post_bias, gate)]
+        s = y.to(wide)
+        if post:
+            s = _torch_norm(s, w[2], w[3], rms, eps)
+        if gate is not None:
+            s = s * w[4]
+        if residual is not None:
+            s = s + alpha * residual.to(wide)
+        h = _torch_norm(s, w[0], w[1], rms, eps).to(y.dtype)
+        return (h, y if plain else s.to(y.dtype if residual is None else residual.dtype)) if return_sum else h
+    if width > _native.lib().resnorm_max_width:
+        raise ValueError(f"residual_norm: a width of {width}: at most {_native.lib().resnorm_max_width} on a GPU")
+    y = y.contiguous()
+    leaves = [None if p is None else p.contiguous()
+              for p in (residual, gate, weight, bias, post_weight, post_bias)]
+    if torch.is_grad_enabled() and any(p is not None and p.requires_grad for p in (y, *leaves)):
+        return _ResidualNormFn.apply(y, *leaves, (gate_rows, post, rms, alpha, eps), return_sum)
+    h, s, _ = _native.lib().resnorm_fwd(y, leaves[0], leaves[1], gate_rows, *leaves[2:], post, rms, alpha, eps,
+                                        return_sum and not plain, False)
+    return (h, y if plain else s) if return_sum else h
+
+
+class ResidualNorm(nn.Module):
+    """``forward(y, residual=None, gate=None, return_sum=False)`` is :func:`residual_norm` with this
+    module's parameters.  ``weight`` and ``bias`` are named as ``nn.LayerNorm``'s, so state dicts of
+    either load into the other; ``post=True`` adds ``post_weight`` (and ``post_bias``)."""
+
+    def __init__(self, width: int, kind: str = "layer", eps: float = 1e-5, bias: bool = True, post: bool = False,
+                 alpha: float = 1.0, device=None, dtype=None):
+        super().__init__()
+        if kind not in ("layer", "rms"):
+            raise ValueError(f"ResidualNorm: kind {kind!r}: 'layer' or 'rms'")
+        self.width, self.kind, self.eps, self.post, self.alpha = width, kind, eps, post, alpha
+        self.weight = nn.Parameter(torch.ones(width, device=device, dtype=dtype))
+        self.bias = nn.Parameter(torch.zeros(width, device=device, dtype=dtype)) if bias else None
+        self.post_weight = nn.Parameter(torch.ones(width, device=device, dtype=dtype)) if post else None
+        self.post_bias = nn.Parameter(torch.zeros(width, device=device, dtype=dtype)) if post and bias else None
+
+    def forward(self, y, residual=None, gate=None, return_sum: bool = False):
+        return residual_norm(y, residual, self.weight, self.bias, kind=self.kind, eps=self.eps, gate=gate,
+                             alpha=self.alpha if residual is not None else 1.0, post=self.post,
+                             post_weight=self.post_weight, post_bias=self.post_bias, return_sum=return_sum)
+
+    def extra_repr(self) -> str:
+        return f"{self.width}, kind={self.kind}, eps={self.eps:g}, post={self.post}, alpha={self.alpha:g}"

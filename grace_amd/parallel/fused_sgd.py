@@ -7,6 +7,10 @@ in the same pass, replacing ``BF16Weights.refresh()`` -- ``DistributedOptimizer(
 weights=w)`` arranges that automatically.  CPU tensors (and ``GRACE_AMD_FORCE_TORCH=1``) run
 ``torch.optim.SGD``'s own functional update.
 
+``max_grad_norm`` clips by the global norm of all gradients of all groups (parallel/clip.py): the
+update kernel multiplies every gradient by the factor as it reads it, so the gradients themselves stay
+as they are.  The norm of the last step is ``opt.grad_norm`` (a 0-dim device tensor).
+
 The learning rate and momentum are read from ``param_groups`` on every ``step()`` call; inside
 a captured HIP graph they are frozen at capture time (as for any host scalar), so LR schedules
 need eager steps or a re-capture.
@@ -41,10 +45,14 @@ def _same_layout(a: torch.Tensor, b: torch.Tensor) -> bool:
 
 class FusedSGD(SGD):
     def __init__(self, params, lr=1e-3, momentum=0.0, dampening=0.0, weight_decay=0.0, nesterov=False, *,
-                 maximize: bool = False):
+                 maximize: bool = False, max_grad_norm: Optional[float] = None):
+        if max_grad_norm is not None and not max_grad_norm >= 0:
+            raise ValueError(f"max_grad_norm {max_grad_norm}: not negative")
         super().__init__(params, lr=lr, momentum=momentum, dampening=dampening, weight_decay=weight_decay,
                          nesterov=nesterov, maximize=maximize)
         self._working: Dict[int, torch.Tensor] = {}
+        self.max_grad_norm = max_grad_norm
+        self.grad_norm: Optional[torch.Tensor] = None
         # the kernel honours the process-wide communication fault flag (parallel/health.py):
         # allocate it now, before any HIP-graph capture of the step
         devs = {p.device for g in self.param_groups for p in g["params"] if p.is_cuda}
@@ -68,6 +76,7 @@ class FusedSGD(SGD):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
+        factor = self._clip_factor() if self.max_grad_norm is not None else None
         for group in self.param_groups:
             native, rest = [], []
             for p in group["params"]:
@@ -80,12 +89,22 @@ class FusedSGD(SGD):
                       and _dense(p))
                 (native if ok else rest).append(p)
             if native:
-                self._native_step(group, native)
+                self._native_step(group, native, factor)
             if rest:
-                self._torch_step(group, rest)
+                self._torch_step(group, rest, factor)
         return loss
 
-    def _native_step(self, group, params):
+    def _clip_factor(self) -> Optional[torch.Tensor]:
+        from .clip import _check, _norm_and_factor, _unique
+
+        grads = _unique([p.grad for g in self.param_groups for p in g["params"] if p.grad is not None])
+        if not grads:
+            return None
+        _check(grads)
+        self.grad_norm, factor = _norm_and_factor(grads, 2, float(self.max_grad_norm))
+        return factor
+
+    def _native_step(self, group, params, factor):
         mom = group["momentum"]
         first, later = [], []
         for p in params:
@@ -105,7 +124,8 @@ class FusedSGD(SGD):
             w16 = [self._working_for(p) for p in ps]
             _native.lib().sgd_step(ps, [p.grad for p in ps], bufs, w16, float(group["lr"]), float(mom),
                                    float(group["dampening"]), float(group["weight_decay"]),
-                                   bool(group["nesterov"]), bool(group.get("maximize", False)), is_first)
+                                   bool(group["nesterov"]), bool(group.get("maximize", False)), is_first,
+                                   None if factor is None else factor.to(dev, torch.float32))
             for p, w in zip(ps, w16):  # working copies the kernel could not write (other strides)
                 if w is None and id(p) in self._working:
                     self._working[id(p)].copy_(p)
@@ -114,11 +134,14 @@ class FusedSGD(SGD):
         w = self._working.get(id(p))
         return w if (w is not None and _same_layout(w, p)) else None
 
-    def _torch_step(self, group, params):
+    def _torch_step(self, group, params, factor):
         from torch.optim.sgd import sgd as functional_sgd
 
         bufs = [self.state[p].get("momentum_buffer") for p in params]
-        functional_sgd(params, [p.grad for p in params], bufs, weight_decay=group["weight_decay"],
+        grads = [p.grad for p in params]
+        if factor is not None:
+            grads = [(g * factor.to(g.device)).to(g.dtype) for g in grads]
+        functional_sgd(params, grads, bufs, weight_decay=group["weight_decay"],
                        momentum=group["momentum"], lr=group["lr"], dampening=group["dampening"],
                        nesterov=group["nesterov"], maximize=group.get("maximize", False), foreach=False)
         if group["momentum"] != 0:
