@@ -60,8 +60,9 @@ struct NormGrads {
   bool bias_f32, post_bias_f32;
 };
 int64_t resnorm_backward_ws(const NormShape& n);  // bytes
-// dh or ds may be null (a zero gradient)
-void resnorm_backward(const NormShape& n, const void* s, const void* y, const float* stats, NormParam gate,
+// s: the sum as it was stored, of type tx = fp32, or y itself without x, gate and post; or nullptr: made again
+// from x (may be null) and y.  dh or ds may be null (a zero gradient).  y may be null where only s is read.
+void resnorm_backward(const NormShape& n, const void* s, const void* x, const void* y, const float* stats, NormParam gate,
                       NormParam weight, NormParam post_weight, NormParam post_bias, const void* dh, const void* ds,
                       const NormGrads& g, void* ws, hipStream_t stream);
 

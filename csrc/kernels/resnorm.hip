@@ -15,8 +15,8 @@ namespace {
 
 using namespace resnorm;
 
-constexpr int kMaxParts = 1024;  // partial rows of the column sums
-constexpr int kMinRows = 4;      // rows per row slot of a workgroup before another workgroup is added
+constexpr int kCUs = 256;
+constexpr int kMinRows = 4;  // rows per row slot of a workgroup before another workgroup is added
 
 struct FoldArgs {
   const float* part;
@@ -54,16 +54,22 @@ __global__ __launch_bounds__(1024) void resnorm_fold_kernel(FoldArgs a) {
 
 int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-// row slots of a workgroup
-int row_slots(int d, bool full) {
-  int slots = 1;
-  by_width(d, full, [&](auto, auto tpr) { slots = block_of<decltype(tpr)::value>() / decltype(tpr)::value; });
-  return slots;
+// row slots of a workgroup, and the workgroups that the chip holds at a time
+struct Shape {
+  int slots, resident;
+};
+Shape shape_of(int d) {
+  Shape s{};
+  by_width(d, [&](auto, auto tpr) {
+    constexpr int TPR = decltype(tpr)::value;
+    s = {block_of<TPR>() / TPR, kCUs * 1024 / block_of<TPR>()};
+  });
+  return s;
 }
 
-Split split_rows(const NormShape& n, bool full, bool grouped) {
-  const int slots = row_slots(n.d, full);
-  const int64_t most = std::max<int64_t>(1, std::min<int64_t>(kMaxParts, cdiv(n.rows, (int64_t)slots * kMinRows)));
+Split split_rows(const NormShape& n, bool grouped) {
+  const Shape shape = shape_of(n.d);
+  const int64_t most = std::max<int64_t>(1, std::min<int64_t>(shape.resident, cdiv(n.rows, (int64_t)shape.slots * kMinRows)));
   Split s{1, n.rows, most, 1, most};
   if (grouped && n.gate_rows < n.rows) {
     s.groups = n.rows / n.gate_rows;
@@ -93,27 +99,25 @@ void resnorm_forward(const NormShape& n, const void* x, const void* y, NormParam
   by_types(n, [&](auto* tag_x, auto* tag_y) {
     using TX = std::remove_pointer_t<decltype(tag_x)>;
     using TY = std::remove_pointer_t<decltype(tag_y)>;
-    launch_forward<TX, TY>(a, stream);
+    launch_forward<TX, TY>(a, 2 * shape_of(n.d).resident, stream);
   });
 }
 
 int64_t resnorm_backward_ws(const NormShape& n) {
-  int64_t blocks = 1;
-  for (bool full : {false, true})
-    for (bool grouped : {false, true}) blocks = std::max(blocks, split_rows(n, full, grouped).blocks);
+  const int64_t blocks = std::max(split_rows(n, false).blocks, split_rows(n, true).blocks);
   return kSums * blocks * n.d * (int64_t)sizeof(float);
 }
 
-void resnorm_backward(const NormShape& n, const void* s, const void* y, const float* stats, NormParam gate,
+void resnorm_backward(const NormShape& n, const void* s, const void* x, const void* y, const float* stats, NormParam gate,
                       NormParam weight, NormParam post_weight, NormParam post_bias, const void* dh, const void* ds,
                       const NormGrads& g, void* ws, hipStream_t stream) {
   if (n.rows == 0 || n.d == 0) return;
-  const bool full = gate.p != nullptr || n.post;
   const bool own_rows = n.gate_rows == 1 && n.rows > 1;  // the gate has the rows' own shape
   BwdArgs a{};
   a.n = n;
-  a.split = split_rows(n, full, g.dgate != nullptr && !own_rows);
+  a.split = split_rows(n, g.dgate != nullptr && !own_rows);
   a.s = s;
+  a.x = x;
   a.y = y;
   a.dh = dh;
   a.ds = ds;
@@ -126,9 +130,11 @@ void resnorm_backward(const NormShape& n, const void* s, const void* y, const fl
   a.dy = g.dy;
   a.dgate = g.dgate;
   a.dgate_f32 = gate.f32;
-  a.dgate_mode = g.dgate == nullptr ? 0 : own_rows ? 3 : a.split.groups > 1 && a.split.parts == 1 ? 2 : 1;
+  a.dgate_mode = g.dgate == nullptr ? kGateNone
+                 : own_rows         ? kGateRows
+                 : a.split.groups > 1 && a.split.parts == 1 ? kGateGroups : kGateParts;
   a.part = static_cast<float*>(ws);
-  void* const outs[kSums] = {g.dweight, g.dbias, a.dgate_mode == 1 ? g.dgate : nullptr, g.dpost_weight, g.dpost_bias};
+  void* const outs[kSums] = {g.dweight, g.dbias, a.dgate_mode == kGateParts ? g.dgate : nullptr, g.dpost_weight, g.dpost_bias};
   FoldArgs f{};
   f.part = a.part;
   f.blocks = a.split.blocks;
@@ -147,7 +153,7 @@ void resnorm_backward(const NormShape& n, const void* s, const void* y, const fl
   by_types(n, [&](auto* tag_x, auto* tag_y) {
     using TX = std::remove_pointer_t<decltype(tag_x)>;
     using TY = std::remove_pointer_t<decltype(tag_y)>;
-    launch_backward<TX, TY>(a, full, stream);
+    launch_backward<TX, TY>(a, stream);
     if (f.sums > 0)
       resnorm_fold_kernel<TY><<<dim3((unsigned)cdiv(n.d, kWave), (unsigned)out_rows), 1024, 0, stream>>>(f);
   });

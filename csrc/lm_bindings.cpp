@@ -6,6 +6,8 @@
 #include <c10/hip/HIPException.h>
 
 #include <algorithm>
+#include <array>
+#include <tuple>
 
 #include "grace_lm.h"
 
@@ -72,14 +74,46 @@ Tensor embed_bwd(const Tensor& ids, const Tensor& dy, int64_t vocab, int64_t pad
   return dw;
 }
 
+// The differentiable calls are C++ autograd functions: a training call costs a few microseconds of host
+// time, where a Python function costs some fifty.  They are differentiable once.
+void once_only(const char* what) {
+  TORCH_CHECK(!at::GradMode::is_enabled(), what, " is differentiable once: no create_graph");
+}
+
+struct EmbeddingFn : torch::autograd::Function<EmbeddingFn> {
+  static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& weight, const Tensor& ids, double scale,
+                        int64_t pad, at::ScalarType dtype) {
+    ctx->save_for_backward({ids});
+    ctx->saved_data["args"] = std::vector<int64_t>{weight.size(0), pad, (int64_t)weight.scalar_type()};
+    ctx->saved_data["scale"] = scale;
+    return embed_fwd(ids, weight, scale, dtype);
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
+                                                 torch::autograd::variable_list grads) {
+    once_only("embedding");
+    const Tensor ids = ctx->get_saved_variables()[0];
+    const auto args = ctx->saved_data["args"].toIntVector();
+    return {embed_bwd(ids, grads[0].contiguous(), args[0], args[1], ctx->saved_data["scale"].toDouble(),
+                      (at::ScalarType)args[2]),
+            Tensor(), Tensor(), Tensor(), Tensor()};
+  }
+};
+
+Tensor embedding(const Tensor& ids, const Tensor& weight, double scale, int64_t pad, at::ScalarType dtype) {
+  const Tensor i = ids.contiguous();
+  const Tensor w = weight.dim() == 2 && weight.stride(1) != 1 && weight.size(1) > 1 ? weight.contiguous() : weight;
+  if (at::GradMode::is_enabled() && w.requires_grad()) return EmbeddingFn::apply(w, i, scale, pad, dtype);
+  return embed_fwd(i, w, scale, dtype);
+}
+
 // ---------------------------------------------------------------- residual norm
-grace::NormParam norm_param(const OptTensor& t, int64_t n, const Tensor& y, const char* what) {
-  if (!has(t)) return {nullptr, false};
-  check_on(*t, y, what);
-  TORCH_CHECK(t->is_contiguous() && t->numel() == n, what, ": contiguous, ", n, " values");
-  TORCH_CHECK(t->scalar_type() == at::kFloat || t->scalar_type() == y.scalar_type(), what,
+grace::NormParam norm_param(const Tensor& t, int64_t n, const Tensor& y, const char* what) {
+  if (!t.defined()) return {nullptr, false};
+  check_on(t, y, what);
+  TORCH_CHECK(t.is_contiguous() && t.numel() == n, what, ": contiguous, ", n, " values");
+  TORCH_CHECK(t.scalar_type() == at::kFloat || t.scalar_type() == y.scalar_type(), what,
               " must be float32 or of the block's type");
-  return {t->data_ptr(), t->scalar_type() == at::kFloat};
+  return {t.data_ptr(), t.scalar_type() == at::kFloat};
 }
 
 grace::NormShape norm_shape(const Tensor& y, at::ScalarType tx, int64_t gate_rows, double alpha, double eps, bool rms,
@@ -88,6 +122,7 @@ grace::NormShape norm_shape(const Tensor& y, at::ScalarType tx, int64_t gate_row
   const int64_t d = y.size(-1);
   TORCH_CHECK(d >= 1 && d <= grace::kNormMaxWidth, "residual norm: widths 1 to ", grace::kNormMaxWidth);
   const int64_t rows = y.numel() / d;
+  TORCH_CHECK(rows < INT32_MAX, "residual norm: at most 2^31 - 2 rows");
   TORCH_CHECK(rows == 0 || (gate_rows >= 1 && rows % gate_rows == 0), "residual norm: rows per gate row");
   grace::NormShape n{rows, gate_rows, (int)d, (float)alpha, (float)eps, rms, post,
                      el_type(tx, "residual norm: the residual"), el_type(y.scalar_type(), "residual norm: the block")};
@@ -95,30 +130,41 @@ grace::NormShape norm_shape(const Tensor& y, at::ScalarType tx, int64_t gate_row
   return n;
 }
 
-int64_t gate_size(const grace::NormShape& n) { return n.rows == 0 ? -1 : n.rows / n.gate_rows * n.d; }
+int64_t gate_size(const grace::NormShape& n) { return n.rows / n.gate_rows * n.d; }
 
-// returns (h, s, stats); s and stats are undefined where they are not wanted
-std::vector<Tensor> resnorm_fwd(const Tensor& y, const OptTensor& x, const OptTensor& gate, int64_t gate_rows,
-                                const OptTensor& weight, const OptTensor& bias, const OptTensor& post_weight,
-                                const OptTensor& post_bias, bool post, bool rms, double alpha, double eps,
-                                bool want_sum, bool want_stats) {
-  const auto tx = has(x) ? x->scalar_type() : y.scalar_type();
-  const grace::NormShape n = norm_shape(y, tx, gate_rows, alpha, eps, rms, post);
-  if (has(x)) {
-    check_on(*x, y, "residual norm: the residual");
-    TORCH_CHECK(x->sizes() == y.sizes() && x->is_contiguous(), "residual norm: the residual must be like the block");
+struct NormTensors {
+  Tensor y, x, gate, weight, bias, post_weight, post_bias;  // undefined: not there
+};
+struct NormOptions {
+  int64_t gate_rows;
+  bool post, rms;
+  double alpha, eps;
+};
+
+// Without a residual, a gate and a post norm the sum is the block itself.
+bool is_plain(const NormTensors& t, const NormOptions& o) { return !t.x.defined() && !t.gate.defined() && !o.post; }
+
+// (h, s, stats); s and stats are undefined where they are not wanted
+std::tuple<Tensor, Tensor, Tensor> resnorm_fwd(const NormTensors& t, const NormOptions& o, bool want_sum,
+                                               bool want_stats) {
+  const Tensor& y = t.y;
+  const auto tx = t.x.defined() ? t.x.scalar_type() : y.scalar_type();
+  const grace::NormShape n = norm_shape(y, tx, o.gate_rows, o.alpha, o.eps, o.rms, o.post);
+  if (t.x.defined()) {
+    check_on(t.x, y, "residual norm: the residual");
+    TORCH_CHECK(t.x.sizes() == y.sizes() && t.x.is_contiguous(), "residual norm: the residual must be like the block");
   }
   DevGuard guard(y.device());
   Tensor h = at::empty_like(y);
   Tensor s = want_sum ? at::empty(y.sizes(), y.options().dtype(tx)) : Tensor();
-  Tensor stats = want_stats ? at::empty({post ? 4 : 2, n.rows}, y.options().dtype(at::kFloat)) : Tensor();
+  Tensor stats = want_stats ? at::empty({o.post ? 4 : 2, n.rows}, y.options().dtype(at::kFloat)) : Tensor();
   if (n.rows > 0) {
-    grace::resnorm_forward(n, has(x) ? x->data_ptr() : nullptr, y.data_ptr(),
-                           norm_param(gate, gate_size(n), y, "residual norm: the gate"),
-                           norm_param(weight, n.d, y, "residual norm: weight"),
-                           norm_param(bias, n.d, y, "residual norm: bias"),
-                           norm_param(post_weight, n.d, y, "residual norm: post_weight"),
-                           norm_param(post_bias, n.d, y, "residual norm: post_bias"), h.data_ptr(),
+    grace::resnorm_forward(n, t.x.defined() ? t.x.data_ptr() : nullptr, y.data_ptr(),
+                           norm_param(t.gate, gate_size(n), y, "residual norm: the gate"),
+                           norm_param(t.weight, n.d, y, "residual norm: weight"),
+                           norm_param(t.bias, n.d, y, "residual norm: bias"),
+                           norm_param(t.post_weight, n.d, y, "residual norm: post_weight"),
+                           norm_param(t.post_bias, n.d, y, "residual norm: post_bias"), h.data_ptr(),
                            want_sum ? s.data_ptr() : nullptr, want_stats ? stats.data_ptr<float>() : nullptr,
                            cur_stream());
     C10_HIP_KERNEL_LAUNCH_CHECK();
@@ -126,48 +172,122 @@ std::vector<Tensor> resnorm_fwd(const Tensor& y, const OptTensor& x, const OptTe
   return {h, s, stats};
 }
 
-// want: dx, dy (always made), dgate, dweight, dbias, dpost_weight, dpost_bias.
-// returns those in that order, undefined where not wanted; one tensor for dx and dy where they are equal
-std::vector<Tensor> resnorm_bwd(const OptTensor& dh, const OptTensor& ds, const Tensor& s, const Tensor& y,
-                                const Tensor& stats, const OptTensor& gate, int64_t gate_rows, const OptTensor& weight,
-                                const OptTensor& bias, const OptTensor& post_weight, const OptTensor& post_bias,
-                                bool post, bool rms, double alpha, double eps, std::vector<bool> want) {
-  const grace::NormShape n = norm_shape(y, s.scalar_type(), gate_rows, alpha, eps, rms, post);
-  TORCH_CHECK(want.size() == 7, "residual norm: seven flags");
-  auto like = [&](const Tensor& t, at::ScalarType type, const char* what) {
-    check_on(t, y, what);
-    TORCH_CHECK(t.sizes() == y.sizes() && t.is_contiguous() && t.scalar_type() == type, what, " must be like the forward's");
+// The gradients of y, x, gate, weight, bias, post_weight, post_bias, undefined where want is not set; one
+// tensor for y and x where they are equal.  s: the stored sum, or undefined: made again from x and y.
+std::vector<Tensor> resnorm_bwd(const Tensor& dh, const Tensor& ds, const NormTensors& t, const NormOptions& o,
+                                const Tensor& s, const Tensor& stats, const std::array<bool, 7>& want,
+                                at::ScalarType tx, at::ScalarType ty) {
+  const Tensor& like = dh.defined() ? dh : ds;
+  const Tensor shape = like.scalar_type() == ty ? like : at::empty(like.sizes(), like.options().dtype(ty));
+  const grace::NormShape n = norm_shape(shape, tx, o.gate_rows, o.alpha, o.eps, o.rms, o.post);
+  auto check = [&](const Tensor& u, at::ScalarType type, const char* what) {
+    if (!u.defined()) return;
+    check_on(u, like, what);
+    TORCH_CHECK(u.sizes() == like.sizes() && u.is_contiguous() && u.scalar_type() == type, what,
+                " must be like the forward's");
   };
-  like(s, s.scalar_type(), "residual norm: the saved sum");
-  if (has(dh)) like(*dh, y.scalar_type(), "residual norm: the norm's gradient");
-  if (has(ds)) like(*ds, s.scalar_type(), "residual norm: the sum's gradient");
+  check(s, tx, "residual norm: the saved sum");
+  check(t.x, tx, "residual norm: the residual");
+  check(t.y, ty, "residual norm: the block");
+  check(dh, ty, "residual norm: the norm's gradient");
+  check(ds, tx, "residual norm: the sum's gradient");
+  TORCH_CHECK(s.defined() || t.y.defined(), "residual norm: neither the sum nor its parts were saved");
+  TORCH_CHECK(t.y.defined() || !(t.gate.defined() || o.post), "residual norm: the block was not saved");
   TORCH_CHECK(stats.is_cuda() && stats.scalar_type() == at::kFloat && stats.is_contiguous() &&
-                  stats.numel() == (post ? 4 : 2) * n.rows, "residual norm: the saved statistics");
-  DevGuard guard(y.device());
-  const grace::NormParam gp = norm_param(gate, gate_size(n), y, "residual norm: the gate");
-  const grace::NormParam wp = norm_param(weight, n.d, y, "residual norm: weight");
-  const grace::NormParam bp = norm_param(bias, n.d, y, "residual norm: bias");
-  const grace::NormParam pwp = norm_param(post_weight, n.d, y, "residual norm: post_weight");
-  const grace::NormParam pbp = norm_param(post_bias, n.d, y, "residual norm: post_bias");
-  auto made = [&](int k, const OptTensor& p) {
-    if (!want[k] || !has(p)) return Tensor();
-    return n.rows > 0 ? at::empty_like(*p) : at::zeros_like(*p);
+                  stats.numel() == (o.post ? 4 : 2) * n.rows, "residual norm: the saved statistics");
+  DevGuard guard(like.device());
+  const grace::NormParam gp = norm_param(t.gate, gate_size(n), shape, "residual norm: the gate");
+  const grace::NormParam wp = norm_param(t.weight, n.d, shape, "residual norm: weight");
+  const grace::NormParam bp = norm_param(t.bias, n.d, shape, "residual norm: bias");
+  const grace::NormParam pwp = norm_param(t.post_weight, n.d, shape, "residual norm: post_weight");
+  const grace::NormParam pbp = norm_param(t.post_bias, n.d, shape, "residual norm: post_bias");
+  auto made = [&](int k, const Tensor& p) {
+    if (!want[k] || !p.defined()) return Tensor();
+    return n.rows > 0 ? at::empty_like(p) : at::zeros_like(p);
   };
-  Tensor dy = at::empty_like(y);
-  const bool one = !gp.p && !post && (float)alpha == 1.f && n.tx == n.ty;
-  Tensor dx = !want[0] ? Tensor() : one ? dy : at::empty_like(s);
-  Tensor dgate = made(2, gate), dw = made(3, weight), db = made(4, bias), dpw = made(5, post_weight),
-         dpb = made(6, post_bias);
+  Tensor dy = at::empty_like(shape);
+  const bool one = !gp.p && !o.post && n.alpha == 1.f && n.tx == n.ty;
+  Tensor dx = !want[1] ? Tensor() : one ? dy : at::empty(like.sizes(), like.options().dtype(tx));
+  Tensor dgate = made(2, t.gate), dw = made(3, t.weight), db = made(4, t.bias), dpw = made(5, t.post_weight),
+         dpb = made(6, t.post_bias);
   if (n.rows > 0) {
-    auto ptr = [](const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; };
+    auto ptr = [](const Tensor& u) { return u.defined() ? u.data_ptr() : nullptr; };
     const grace::NormGrads g{ptr(dx), dy.data_ptr(), ptr(dgate), ptr(dw), ptr(db), ptr(dpw), ptr(dpb), bp.f32, pbp.f32};
-    Tensor ws = at::empty({grace::resnorm_backward_ws(n)}, y.options().dtype(at::kByte));
-    grace::resnorm_backward(n, s.data_ptr(), y.data_ptr(), stats.data_ptr<float>(), gp, wp, pwp, pbp,
-                            has(dh) ? dh->data_ptr() : nullptr, has(ds) ? ds->data_ptr() : nullptr, g, ws.data_ptr(),
-                            cur_stream());
+    Tensor ws = at::empty({grace::resnorm_backward_ws(n)}, like.options().dtype(at::kByte));
+    grace::resnorm_backward(n, ptr(s), ptr(t.x), ptr(t.y), stats.data_ptr<float>(), gp, wp, pwp, pbp, ptr(dh), ptr(ds),
+                            g, ws.data_ptr(), cur_stream());
     C10_HIP_KERNEL_LAUNCH_CHECK();
   }
-  return {dx, dy, dgate, dw, db, dpw, dpb};
+  return {want[0] ? dy : Tensor(), dx, dgate, dw, db, dpw, dpb};
+}
+
+struct ResidualNormFn : torch::autograd::Function<ResidualNormFn> {
+  static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const Tensor& y,
+                                                const OptTensor& ox, const OptTensor& ogate, const OptTensor& oweight,
+                                                const OptTensor& obias, const OptTensor& opost_weight,
+                                                const OptTensor& opost_bias, const NormOptions& o, bool return_sum) {
+    auto get = [](const OptTensor& t) { return has(t) ? *t : Tensor(); };
+    const Tensor x = get(ox), gate = get(ogate), weight = get(oweight), bias = get(obias),
+                 post_weight = get(opost_weight), post_bias = get(opost_bias);
+    const NormTensors t{y, x, gate, weight, bias, post_weight, post_bias};
+    const auto tx = x.defined() ? x.scalar_type() : y.scalar_type();
+    const bool plain = is_plain(t, o), stored = !plain && tx == at::kFloat;
+    auto [h, s, stats] = resnorm_fwd(t, o, !plain && (return_sum || stored), true);
+    const bool keeps_y = gate.defined() || o.post || !(plain || stored);
+    ctx->save_for_backward({plain ? y : stored ? s : Tensor(), plain || stored ? Tensor() : x, keeps_y ? y : Tensor(),
+                            gate, weight, bias, post_weight, post_bias, stats});
+    ctx->saved_data["ints"] = std::vector<int64_t>{o.gate_rows, o.post, o.rms, (int64_t)tx, (int64_t)y.scalar_type(),
+                                                  x.defined()};
+    ctx->saved_data["alpha"] = o.alpha;
+    ctx->saved_data["eps"] = o.eps;
+    ctx->set_materialize_grads(false);
+    if (!return_sum) return {h};
+    // the plain sum is an output of its own: its gradient joins the norm's before the one rounding
+    return {h, plain ? y.detach() : s};
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
+                                                 torch::autograd::variable_list grads) {
+    once_only("residual norm");
+    torch::autograd::variable_list out(9);
+    const Tensor dh = grads[0].defined() ? grads[0].contiguous() : Tensor();
+    const Tensor ds = grads.size() > 1 && grads[1].defined() ? grads[1].contiguous() : Tensor();
+    if (!dh.defined() && !ds.defined()) return out;
+    const auto v = ctx->get_saved_variables();
+    const auto i = ctx->saved_data["ints"].toIntVector();
+    const NormOptions o{i[0], i[1] != 0, i[2] != 0, ctx->saved_data["alpha"].toDouble(), ctx->saved_data["eps"].toDouble()};
+    // only the tensors that are there have an edge
+    const std::array<bool, 7> there{true,           i[5] != 0,      v[3].defined(), v[4].defined(),
+                                    v[5].defined(), v[6].defined(), v[7].defined()};
+    std::array<bool, 7> want;
+    for (size_t k = 0, edge = 0; k < want.size(); ++k) want[k] = there[k] && ctx->needs_input_grad(edge++);
+    const auto g = resnorm_bwd(dh, ds, {v[2], v[1], v[3], v[4], v[5], v[6], v[7]}, o, v[0], v[8], want,
+                               (at::ScalarType)i[3], (at::ScalarType)i[4]);
+    std::copy(g.begin(), g.end(), out.begin());
+    return out;
+  }
+};
+
+// h, and s with return_sum
+std::vector<Tensor> residual_norm(const Tensor& y, const OptTensor& x, const OptTensor& gate, int64_t gate_rows,
+                                  const OptTensor& weight, const OptTensor& bias, const OptTensor& post_weight,
+                                  const OptTensor& post_bias, bool post, bool rms, double alpha, double eps,
+                                  bool return_sum) {
+  auto get = [](const OptTensor& t) { return has(t) ? t->contiguous() : Tensor(); };
+  const NormTensors t{y.contiguous(), get(x), get(gate), get(weight), get(bias), get(post_weight), get(post_bias)};
+  const NormOptions o{gate_rows, post, rms, alpha, eps};
+  bool grad = false;
+  if (at::GradMode::is_enabled())
+    for (const Tensor* p : {&t.y, &t.x, &t.gate, &t.weight, &t.bias, &t.post_weight, &t.post_bias})
+      grad |= p->defined() && p->requires_grad();
+  if (grad) {
+    auto opt = [](const Tensor& u) { return u.defined() ? OptTensor(u) : OptTensor(); };
+    return ResidualNormFn::apply(t.y, opt(t.x), opt(t.gate), opt(t.weight), opt(t.bias), opt(t.post_weight),
+                                 opt(t.post_bias), o, return_sum);
+  }
+  const bool plain = is_plain(t, o);
+  auto [h, s, stats] = resnorm_fwd(t, o, return_sum && !plain, false);
+  if (!return_sum) return {h};
+  return {h, plain ? t.y : s};
 }
 
 // ---------------------------------------------------------------- global gradient norm
@@ -244,17 +364,32 @@ void grad_scale(const std::vector<Tensor>& grads, const Tensor& factor) {
   const auto g = grad_list(grads);
   grace::grad_scale(g.data(), (int64_t)g.size(), factor.data_ptr<float>(), cur_stream());
   C10_HIP_KERNEL_LAUNCH_CHECK();
+  for (const Tensor& t : grads) t.unsafeGetTensorImpl()->bump_version();
 }
 
-// norm, factor and scaling of tensors of one GPU; returns [norm, factor]
-Tensor grad_clip(const std::vector<Tensor>& grads, int64_t kind, double max_norm) {
-  TORCH_CHECK(!grads.empty(), "gradient norm: no tensors");
+// [norm, factor] fp32 of the parameters' gradients, which are scaled in place with `scale`; none where they
+// are not all dense gradients of a kernel's type on one GPU, or not there
+OptTensor grad_clip(const std::vector<Tensor>& params, int64_t kind, double max_norm, bool scale) {
+  std::vector<Tensor> grads;
+  grads.reserve(params.size());
+  for (const Tensor& p : params) {
+    const Tensor& g = p.grad();
+    if (!g.defined()) continue;
+    const auto t = g.scalar_type();
+    if (!g.is_cuda() || g.layout() != at::kStrided || (t != at::kFloat && t != at::kBFloat16 && t != at::kHalf) ||
+        (!grads.empty() && g.device() != grads[0].device()) || !g.is_non_overlapping_and_dense())
+      return c10::nullopt;
+    grads.push_back(g);
+  }
+  if (grads.empty()) return c10::nullopt;
   DevGuard guard(grads[0].device());
   const auto g = grad_list(grads);
-  Tensor part = parts_of(g, norm_kind(kind), grads[0]);
-  Tensor out = grad_norm_finish(part, kind, max_norm);
-  grace::grad_scale(g.data(), (int64_t)g.size(), out.data_ptr<float>() + 1, cur_stream());
-  C10_HIP_KERNEL_LAUNCH_CHECK();
+  Tensor out = grad_norm_finish(parts_of(g, norm_kind(kind), grads[0]), kind, max_norm);
+  if (scale) {
+    grace::grad_scale(g.data(), (int64_t)g.size(), out.data_ptr<float>() + 1, cur_stream());
+    C10_HIP_KERNEL_LAUNCH_CHECK();
+    for (const Tensor& t : grads) t.unsafeGetTensorImpl()->bump_version();
+  }
   return out;
 }
 
@@ -265,14 +400,11 @@ at::ScalarType scalar_type(const py::object& dtype) {
 }  // namespace
 
 void grace_bind_lm(py::module& m) {
-  m.def("embed_fwd", [](const Tensor& ids, const Tensor& weight, double scale, const py::object& dtype) {
-    return embed_fwd(ids, weight, scale, scalar_type(dtype));
+  m.def("embedding", [](const Tensor& ids, const Tensor& weight, double scale, int64_t pad, const py::object& dtype) {
+    return embedding(ids, weight, scale, pad, scalar_type(dtype));
   });
-  m.def("embed_bwd", [](const Tensor& ids, const Tensor& dy, int64_t vocab, int64_t pad, double scale,
-                        const py::object& dtype) { return embed_bwd(ids, dy, vocab, pad, scale, scalar_type(dtype)); });
   m.attr("resnorm_max_width") = (int64_t)grace::kNormMaxWidth;
-  m.def("resnorm_fwd", &resnorm_fwd);
-  m.def("resnorm_bwd", &resnorm_bwd);
+  m.def("residual_norm", &residual_norm);
   m.def("grad_norm_parts", &grad_norm_parts);
   m.def("grad_norm_finish", &grad_norm_finish);
   m.def("grad_scale", &grad_scale);

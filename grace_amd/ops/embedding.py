@@ -16,26 +16,10 @@ from typing import Optional
 import torch
 import torch.nn as nn
 import torch.nn.functional as F
-from torch.autograd.function import once_differentiable
 
 from . import _native
 
 _DTYPES = (torch.float32, torch.bfloat16, torch.float16)
-
-
-class _EmbeddingFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, weight, ids, scale, pad, dtype):
-        ctx.save_for_backward(ids)
-        ctx.args = (weight.shape[0], pad, scale, weight.dtype)
-        return _native.lib().embed_fwd(ids, weight, scale, dtype)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dy):
-        (ids,) = ctx.saved_tensors
-        vocab, pad, scale, dtype = ctx.args
-        return _native.lib().embed_bwd(ids, dy.contiguous(), vocab, pad, scale, dtype), None, None, None, None
 
 
 def embedding(ids: torch.Tensor, weight: torch.Tensor, scale: float = 1.0, padding_idx: Optional[int] = None,
@@ -65,12 +49,7 @@ def embedding(ids: torch.Tensor, weight: torch.Tensor, scale: float = 1.0, paddi
             raise TypeError(f"embedding: float32, bfloat16 or float16 on a GPU, got {weight.dtype} -> {dtype}")
         if ids.numel() >= 2**31 - 1 or rows >= 2**31 - 1:
             raise ValueError("embedding: at most 2^31 - 2 tokens and rows")
-        ids = ids.contiguous()
-        if weight.stride(1) != 1 and weight.shape[1] > 1:
-            weight = weight.contiguous()
-        if torch.is_grad_enabled() and weight.requires_grad:
-            return _EmbeddingFn.apply(weight, ids, float(scale), pad, dtype)
-        return _native.lib().embed_fwd(ids, weight, float(scale), dtype)
+        return _native.lib().embedding(ids, weight, float(scale), pad, dtype)
     wide = weight if weight.dtype == torch.float64 else weight.float()
     return (F.embedding(ids, wide, None if pad < 0 else pad) * float(scale)).to(dtype)
 

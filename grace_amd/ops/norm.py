@@ -10,8 +10,9 @@ of the last dimension,
 with N a layer norm or a root-mean-square norm.  Without options it is a plain norm of ``y``; with a
 residual alone it is the post-norm step ``N(x + f(x))`` of the encoder.  Everything is computed in fp32
 (fp64 for fp64 inputs on the CPU) from the unrounded sum; ``h`` has the type of ``y``, ``s`` that of ``x``.
-The backward is one pass too: it reads ``s`` (and ``y`` where a gate or a post norm needs it), and the
-gradients of weights, biases and shared gates are summed in a fixed order.
+The backward is one pass too: it keeps an fp32 ``s`` (and ``y`` where a gate or a post norm needs it), or
+``x`` and ``y`` where the sum would be rounded to 16 bits; the gradients of weights, biases and shared
+gates are summed in a fixed order.
 """
 from __future__ import annotations
 
@@ -19,45 +20,10 @@ from typing import Optional
 
 import torch
 import torch.nn as nn
-from torch.autograd.function import once_differentiable
 
 from . import _native
 
 _DTYPES = (torch.float32, torch.bfloat16, torch.float16)
-
-
-class _ResidualNormFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, y, x, gate, weight, bias, post_weight, post_bias, args, return_sum):
-        gate_rows, post, rms, alpha, eps = args
-        plain = x is None and gate is None and not post
-        h, s, stats = _native.lib().resnorm_fwd(y, x, gate, gate_rows, weight, bias, post_weight, post_bias, post,
-                                                rms, alpha, eps, not plain, True)
-        uses_y = gate is not None or post
-        ctx.save_for_backward(y if plain else s, y if uses_y else None, stats, gate, weight, bias, post_weight,
-                              post_bias)
-        ctx.args = args
-        ctx.dtype = y.dtype
-        ctx.set_materialize_grads(False)
-        # without residual, gate and post norm the sum is the block itself, as an output of its own: its
-        # gradient then joins the norm's before the one rounding
-        return (h, y.detach() if plain else s) if return_sum else h
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dh, ds=None):
-        if dh is None and ds is None:
-            return (None,) * 9
-        s, y, stats, gate, weight, bias, post_weight, post_bias = ctx.saved_tensors
-        gate_rows, post, rms, alpha, eps = ctx.args
-        dh = None if dh is None else dh.contiguous()
-        ds = None if ds is None else ds.contiguous()
-        if y is None:  # only its type and shape count
-            y = dh if dh is not None else torch.empty(s.shape, dtype=ctx.dtype, device=s.device)
-        need = ctx.needs_input_grad
-        dx, dy, *rest = _native.lib().resnorm_bwd(dh, ds, s, y, stats, gate, gate_rows, weight, bias, post_weight,
-                                                  post_bias, post, rms, alpha, eps, [need[1], need[0], *need[2:7]])
-        return (dy if need[0] else None, dx, *rest, None, None)
 
 
 def _gate_rows(gate: torch.Tensor, y: torch.Tensor) -> int:
@@ -147,14 +113,9 @@ def residual_norm(y: torch.Tensor, residual: Optional[torch.Tensor] = None, weig
         return (h, y if plain else s.to(y.dtype if residual is None else residual.dtype)) if return_sum else h
     if width > _native.lib().resnorm_max_width:
         raise ValueError(f"residual_norm: a width of {width}: at most {_native.lib().resnorm_max_width} on a GPU")
-    y = y.contiguous()
-    leaves = [None if p is None else p.contiguous()
-              for p in (residual, gate, weight, bias, post_weight, post_bias)]
-    if torch.is_grad_enabled() and any(p is not None and p.requires_grad for p in (y, *leaves)):
-        return _ResidualNormFn.apply(y, *leaves, (gate_rows, post, rms, alpha, eps), return_sum)
-    h, s, _ = _native.lib().resnorm_fwd(y, leaves[0], leaves[1], gate_rows, *leaves[2:], post, rms, alpha, eps,
-                                        return_sum and not plain, False)
-    return (h, y if plain else s) if return_sum else h
+    out = _native.lib().residual_norm(y, residual, gate, gate_rows, weight, bias, post_weight, post_bias, post, rms,
+                                      alpha, eps, return_sum)
+    return tuple(out) if return_sum else out[0]
 
 
 class ResidualNorm(nn.Module):

@@ -113,8 +113,6 @@ def _scale(grads: List[torch.Tensor], factor: torch.Tensor) -> None:
 
 
 def _grads_of(parameters) -> List[torch.Tensor]:
-    if isinstance(parameters, torch.Tensor):
-        parameters = [parameters]
     grads = _unique([p.grad for p in parameters if p.grad is not None])
     _check(grads)
     if any(s == 0 and n > 1 for g in grads for s, n in zip(g.stride(), g.shape)):
@@ -142,13 +140,14 @@ def clip_grad_norm_(parameters: Union[torch.Tensor, Iterable[torch.Tensor]], max
     norm makes the gradients NaN or zero, as torch's function does; ``error_if_nonfinite`` raises instead,
     before anything is scaled, for which it waits for the device."""
     kind, max_norm = _kind(norm_type), float(max_norm)
+    parameters = [parameters] if isinstance(parameters, torch.Tensor) else list(parameters)
+    if not error_if_nonfinite and parameters and _native.use_native(parameters[0]):
+        out = _native.lib().grad_clip(parameters, kind, max_norm, True)
+        if out is not None:
+            return out[0]
     grads = _grads_of(parameters)
     if not grads:
         return torch.tensor(0.0)
-    dev = grads[0].device
-    if not error_if_nonfinite and all(
-            g.device == dev and _native_ok(g) and _dense(g) for g in grads):
-        return _native.lib().grad_clip(grads, kind, max_norm)[0]
     norm, factor = _norm_and_factor(grads, kind, max_norm)
     if error_if_nonfinite and not bool(torch.isfinite(norm)):
         raise RuntimeError(f"The total norm of order {float(norm_type)} for gradients is non-finite, so it cannot be "

@@ -97,7 +97,13 @@ class FusedSGD(SGD):
     def _clip_factor(self) -> Optional[torch.Tensor]:
         from .clip import _check, _norm_and_factor, _unique
 
-        grads = _unique([p.grad for g in self.param_groups for p in g["params"] if p.grad is not None])
+        params = [p for g in self.param_groups for p in g["params"]]
+        if _native.use_native(params[0]):
+            out = _native.lib().grad_clip(params, 2, float(self.max_grad_norm), False)
+            if out is not None:
+                self.grad_norm = out[0]
+                return out[1]
+        grads = _unique([p.grad for p in params if p.grad is not None])
         if not grads:
             return None
         _check(grads)
