@@ -22,6 +22,7 @@
 #pragma once
 
 #include <algorithm>
+#include <atomic>
 #include <type_traits>
 
 #include "grace_common.h"
@@ -29,6 +30,8 @@
 
 namespace grace {
 namespace resnorm {
+
+constexpr int kCUs = 256;
 
 template <int TPR>
 constexpr int block_of() { return TPR < 256 ? 256 : TPR; }
@@ -122,7 +125,7 @@ struct RowSum {
 
 template <typename T, int V, int J>
 struct Raw {
-  Pack<T, V> v[J];
+  Bits<T, V> v[J];
 };
 
 template <int TPR, int V, int J>
@@ -141,14 +144,8 @@ struct Row {
 #pragma unroll
     for (int j = 0; j < J; ++j) {
 #pragma unroll
-      for (int i = 0; i < V; ++i) r.v[j].v[i] = (T)0.f;
-      const T* q = static_cast<const T*>(p) + at + col(j);
-      if (p != nullptr && left[j] >= V) r.v[j] = *reinterpret_cast<const Pack<T, V>*>(q);
-      else if (p != nullptr && left[j] > 0) {
-#pragma unroll
-        for (int i = 0; i < V; ++i)
-          if (i < left[j]) r.v[j].v[i] = q[i];
-      }
+      for (int i = 0; i < Bits<T, V>::W; ++i) r.v[j].w[i] = 0;
+      if (p != nullptr && left[j] > 0) load_bits(static_cast<const T*>(p) + at + col(j), r.v[j], left[j]);
     }
   }
   template <typename TY>
@@ -207,11 +204,73 @@ struct Row {
   }
 };
 
+// The weights (and in the backward the gate) of a workgroup's rows, each thread's own values.  Rows that
+// take a workgroup keep them in LDS, where they cost no registers: the registers decide how many such
+// rows a CU has in flight.  Only the thread that wrote a value reads it, so there are no barriers.
+// 16384 columns would take 64 KB an array, so rows of 16 values a thread keep them in registers.
+template <int K, int TPR, int V, int J, bool LDS>
+struct Params {
+  static constexpr bool kLds = LDS;
+  static constexpr int kFloats = kLds ? TPR * V * J : 0;  // of LDS, for each array
+  float r[kLds ? 1 : K][J][V];
+  float4* lds;
+  __device__ __forceinline__ explicit Params(float* p) : lds(reinterpret_cast<float4*>(p) + threadIdx.x) {}
+  // k: the array (a constant), at: its place in LDS
+  __device__ __forceinline__ void set(int k, int at, const float (&v)[J][V]) {
+#pragma unroll
+    for (int j = 0; j < J; ++j)
+#pragma unroll
+      for (int i = 0; i < V; i += 4) {
+        if constexpr (kLds) {
+          lds[((at * J + j) * (V / 4) + i / 4) * TPR] = make_float4(v[j][i], v[j][i + 1], v[j][i + 2], v[j][i + 3]);
+        } else {
+#pragma unroll
+          for (int q = 0; q < 4; ++q) r[k][j][i + q] = v[j][i + q];
+        }
+      }
+  }
+  __device__ __forceinline__ void get(int k, int at, float (&v)[J][V]) const {
+#pragma unroll
+    for (int j = 0; j < J; ++j)
+#pragma unroll
+      for (int i = 0; i < V; i += 4) {
+        if constexpr (kLds) {
+          const float4 q = lds[((at * J + j) * (V / 4) + i / 4) * TPR];
+          v[j][i] = q.x;
+          v[j][i + 1] = q.y;
+          v[j][i + 2] = q.z;
+          v[j][i + 3] = q.w;
+        } else {
+#pragma unroll
+          for (int q = 0; q < 4; ++q) v[j][i + q] = r[k][j][i + q];
+        }
+      }
+  }
+};
+
 // the workgroup's slot of rows, known to be the same in a wave
 template <int TPR>
 __device__ __forceinline__ int row_slot() {
   return block_of<TPR>() == TPR ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x / TPR);
 }
+
+enum { kW, kB, kPw, kPb, kG, kParams };
+
+// Which arrays there are, and their places in LDS (-1: not there).
+struct ParamPlaces {
+  int at[kParams], n = 0;
+  __host__ __device__ __forceinline__ ParamPlaces(const void* w, const void* b, const void* gate, const void* pw,
+                                                  const void* pb) {
+    const void* p[kParams] = {w, b, pw, pb, gate};
+#pragma unroll
+    for (int k = 0; k < kParams; ++k) at[k] = p[k] != nullptr ? n++ : -1;
+  }
+};
+
+template <int E, int TPR>
+constexpr bool lds_forward() { return TPR > kWave && TPR < 1024; }  // at most five arrays: 80 KB
+template <int E, int TPR>
+constexpr bool lds_backward() { return TPR > kWave && E == 8; }  // at most four: 128 KB
 
 #define GRACE_EACH(body)          \
   _Pragma("unroll") for (int j = 0; j < J; ++j) \
@@ -228,40 +287,69 @@ __global__ __launch_bounds__(block_of<TPR>()) void resnorm_fwd_kernel(FwdArgs g)
   const uint32_t rows = (uint32_t)n.rows, step = gridDim.x * kSlots, gate_rows = (uint32_t)n.gate_rows;
   uint32_t r = blockIdx.x * kSlots + row_slot<TPR>();
   if (r >= rows) return;
+  // Rows of one wave: many are in flight anyway, and few registers (78 for 160) let all 4096 rows of a
+  // small batch run at once; their weights come from the caches.
+  constexpr bool AHEAD = TPR > kWave;
   Raw<TY, V, J> ry;
   Raw<TX, V, J> rx;
-  row.load(g.y, (int64_t)r * n.d, ry);
-  row.load(g.x, (int64_t)r * n.d, rx);
-  float w[J][V], b[J][V], pw[J][V], pb[J][V], gate[J][V];
-  row.template param<TY>(g.weight, 0, 1.f, w);
-  row.template param<TY>(g.bias, 0, 0.f, b);
-  if (n.post) {
-    row.template param<TY>(g.post_weight, 0, 1.f, pw);
-    row.template param<TY>(g.post_bias, 0, 0.f, pb);
+  auto fetch = [&](uint32_t q) {
+    row.load(g.y, (int64_t)q * n.d, ry);
+    row.load(g.x, (int64_t)q * n.d, rx);
+  };
+  fetch(r);
+  extern __shared__ __align__(16) float dyn[];
+  Params<kParams, TPR, V, J, lds_forward<E, TPR>()> params(dyn);
+  const ParamPlaces at_lds(g.weight.p, g.bias.p, g.gate.p, n.post ? g.post_weight.p : nullptr,
+                           n.post ? g.post_bias.p : nullptr);
+  {
+    float v[J][V];
+    auto put = [&](int k, const NormParam& p, float none) {
+      if (!AHEAD || at_lds.at[k] < 0) return;
+      row.template param<TY>(p, 0, none, v);
+      params.set(k, at_lds.at[k], v);
+    };
+    put(kW, g.weight, 1.f);
+    put(kB, g.bias, 0.f);
+    put(kPw, g.post_weight, 1.f);
+    put(kPb, g.post_bias, 0.f);
   }
+  auto take = [&](int k, const NormParam& from, float(&v)[J][V]) {
+    if constexpr (AHEAD) params.get(k, at_lds.at[k], v);
+    else row.template param<TY>(from, 0, 0.f, v);
+  };
   uint32_t gate_now = ~0u;
   for (;;) {
     const int64_t at = (int64_t)r * n.d;
-    if (g.gate.p != nullptr && r / gate_rows != gate_now) {
+    float u[J][V], x[J][V], p[J][V], gate[J][V], mean, rstd;
+    // a gate that stays is not loaded again: a load here would make the row wait for the last one's stores
+    if (g.gate.p != nullptr && (!AHEAD || r / gate_rows != gate_now)) {
       gate_now = r / gate_rows;
       row.template param<TY>(g.gate, (int64_t)gate_now * n.d, 1.f, gate);
+      if (AHEAD) params.set(kG, at_lds.at[kG], gate);
     }
-    float u[J][V], x[J][V], mean, rstd;
-    GRACE_EACH(u[j][i] = (float)ry.v[j].v[i]; x[j][i] = (float)rx.v[j].v[i])
+    GRACE_EACH(u[j][i] = bits_at(ry.v[j], i); x[j][i] = bits_at(rx.v[j], i))
     const bool more = rows - r > step;
-    if (more) {
-      row.load(g.y, at + (int64_t)step * n.d, ry);
-      row.load(g.x, at + (int64_t)step * n.d, rx);
-    }
+    if (AHEAD && more) fetch(r + step);
     if (n.post) {
       row.stats(u, n.rms, n.eps, sum, mean, rstd);
       if (g.stats != nullptr && row.t == 0) {
         g.stats[2 * n.rows + r] = mean;
         g.stats[3 * n.rows + r] = rstd;
       }
-      GRACE_EACH(u[j][i] = (u[j][i] - mean) * rstd * pw[j][i] + pb[j][i])
+      GRACE_EACH(u[j][i] = (u[j][i] - mean) * rstd)
+      if (g.post_weight.p != nullptr) {
+        take(kPw, g.post_weight, p);
+        GRACE_EACH(u[j][i] *= p[j][i])
+      }
+      if (g.post_bias.p != nullptr) {
+        take(kPb, g.post_bias, p);
+        GRACE_EACH(u[j][i] += p[j][i])
+      }
     }
-    if (g.gate.p != nullptr) GRACE_EACH(u[j][i] *= gate[j][i])
+    if (g.gate.p != nullptr) {
+      if (AHEAD) params.get(kG, at_lds.at[kG], gate);
+      GRACE_EACH(u[j][i] *= gate[j][i])
+    }
     if (g.x != nullptr) GRACE_EACH(u[j][i] = fmaf(n.alpha, x[j][i], u[j][i]))
     row.trim(u);
     if (g.s != nullptr) row.template store<TX>(g.s, at, u);
@@ -270,10 +358,19 @@ __global__ __launch_bounds__(block_of<TPR>()) void resnorm_fwd_kernel(FwdArgs g)
       g.stats[r] = mean;
       g.stats[n.rows + r] = rstd;
     }
-    GRACE_EACH(u[j][i] = (u[j][i] - mean) * rstd * w[j][i] + b[j][i])
+    GRACE_EACH(u[j][i] = (u[j][i] - mean) * rstd)
+    if (g.weight.p != nullptr) {
+      take(kW, g.weight, p);
+      GRACE_EACH(u[j][i] *= p[j][i])
+    }
+    if (g.bias.p != nullptr) {
+      take(kB, g.bias, p);
+      GRACE_EACH(u[j][i] += p[j][i])
+    }
     row.template store<TY>(g.h, at, u);
     if (!more) return;
     r += step;
+    if (!AHEAD) fetch(r);
   }
 }
 
@@ -310,8 +407,9 @@ __device__ __forceinline__ void over_slots(const float (&acc)[J][V], const Row<T
   }
 }
 
-template <typename TX, typename TY, int E, int TPR, bool POST, bool GATED>
-__global__ __launch_bounds__(block_of<TPR>()) void resnorm_bwd_kernel(BwdArgs g) {
+// BIAS: one of the two biases is there
+template <typename TX, typename TY, int E, int TPR, bool POST, bool GATED, bool BIAS>
+__global__ __launch_bounds__(block_of<TPR>(), TPR == 512 ? 4 : 1) void resnorm_bwd_kernel(BwdArgs g) {
   constexpr int V = vec_of<TX, TY>(), J = E / V, kSlots = block_of<TPR>() / TPR;
   constexpr bool AHEAD = TPR > kWave;  // the next row's loads are issued before this row's sums
   __shared__ float scratch[TPR > kWave ? 4 * TPR / kWave : 1];
@@ -319,12 +417,31 @@ __global__ __launch_bounds__(block_of<TPR>()) void resnorm_bwd_kernel(BwdArgs g)
   RowSum<TPR> sum{scratch};
   const NormShape& n = g.n;
   const Row<TPR, V, J> row(threadIdx.x % TPR, n.d);
-  float dw[J][V], db[J][V], dg[J][V], dpw[J][V], dpb[J][V], w[J][V], pw[J][V], pb[J][V], gate[J][V];
+  float dw[J][V], db[J][V], dg[J][V], dpw[J][V], dpb[J][V];
   GRACE_EACH(dw[j][i] = db[j][i] = dg[j][i] = dpw[j][i] = dpb[j][i] = 0.f)
-  row.template param<TY>(g.weight, 0, 1.f, w);
-  if constexpr (POST) {
-    row.template param<TY>(g.post_weight, 0, 1.f, pw);
-    row.template param<TY>(g.post_bias, 0, 0.f, pb);
+  extern __shared__ __align__(16) float dyn[];
+  Params<2 + 2 * POST, TPR, V, J, lds_backward<E, TPR>()> params(dyn);
+  constexpr int W = 0, G = 1, PW = 2, PB = 3;  // the places in registers
+  const ParamPlaces at_lds(g.weight.p, nullptr, g.gate.p, POST ? g.post_weight.p : nullptr,
+                           POST && BIAS ? g.post_bias.p : nullptr);
+  {
+    float v[J][V];
+    if (g.weight.p != nullptr) {
+      row.template param<TY>(g.weight, 0, 1.f, v);
+      params.set(W, at_lds.at[kW], v);
+    }
+    if constexpr (POST) {
+      if (g.post_weight.p != nullptr) {
+        row.template param<TY>(g.post_weight, 0, 1.f, v);
+        params.set(PW, at_lds.at[kPw], v);
+      }
+      if constexpr (BIAS) {
+        if (g.post_bias.p != nullptr) {
+          row.template param<TY>(g.post_bias, 0, 0.f, v);
+          params.set(PB, at_lds.at[kPb], v);
+        }
+      }
+    }
   }
   const bool again = sizeof(TX) == 2 && g.s == nullptr;
   const void* sx = again ? g.x : g.s;
@@ -357,21 +474,49 @@ __global__ __launch_bounds__(block_of<TPR>()) void resnorm_bwd_kernel(BwdArgs g)
       if constexpr (GATED) {
         if (r / gate_rows != gate_now) {
           gate_now = r / gate_rows;
-          row.template param<TY>(g.gate, (int64_t)gate_now * n.d, 1.f, gate);
+          float v[J][V];
+          row.template param<TY>(g.gate, (int64_t)gate_now * n.d, 1.f, v);
+          params.set(G, at_lds.at[kG], v);
         }
       }
-      float S[J][V], hat[J][V], phat[J][V], ds[J][V];
+      float S[J][V], hat[J][V], phat[J][V], ds[J][V], p[J][V];
+      // u of the forward, without its gate, from phat
+      auto made_u = [&](float(&u)[J][V]) {
+        GRACE_EACH(u[j][i] = phat[j][i])
+        if constexpr (POST) {
+          if (g.post_weight.p != nullptr) {
+            params.get(PW, at_lds.at[kPw], p);
+            GRACE_EACH(u[j][i] *= p[j][i])
+          }
+          if constexpr (BIAS) {
+            if (g.post_bias.p != nullptr) {
+              params.get(PB, at_lds.at[kPb], p);
+              GRACE_EACH(u[j][i] += p[j][i])
+            }
+          }
+        }
+      };
       float c1 = 0.f, c2 = 0.f;
-      GRACE_EACH(phat[j][i] = (float)ry.v[j].v[i]; hat[j][i] = (float)rs.v[j].v[i]; S[j][i] = (float)rdh.v[j].v[i];
-                 ds[j][i] = (float)rds.v[j].v[i])
+      GRACE_EACH(phat[j][i] = bits_at(ry.v[j], i); hat[j][i] = bits_at(rs.v[j], i); S[j][i] = bits_at(rdh.v[j], i);
+                 ds[j][i] = bits_at(rds.v[j], i))
       if (AHEAD && r + kSlots < r_end) fetch(r + kSlots);
       if constexpr (POST) GRACE_EACH(phat[j][i] = (phat[j][i] - pmean) * prstd)
       if (again) {
-        GRACE_EACH(float u = phat[j][i]; if constexpr (POST) u = u * pw[j][i] + pb[j][i];
-                   if constexpr (GATED) u *= gate[j][i]; hat[j][i] = fmaf(n.alpha, hat[j][i], u))
+        float u[J][V];
+        made_u(u);
+        if constexpr (GATED) {
+          params.get(G, at_lds.at[kG], p);
+          GRACE_EACH(u[j][i] *= p[j][i])
+        }
+        GRACE_EACH(hat[j][i] = fmaf(n.alpha, hat[j][i], u[j][i]))
       }
-      GRACE_EACH(hat[j][i] = (hat[j][i] - mean) * rstd; dw[j][i] = fmaf(S[j][i], hat[j][i], dw[j][i]);
-                 db[j][i] += S[j][i]; S[j][i] *= w[j][i]; c1 += S[j][i]; c2 = fmaf(S[j][i], hat[j][i], c2))
+      GRACE_EACH(hat[j][i] = (hat[j][i] - mean) * rstd; dw[j][i] = fmaf(S[j][i], hat[j][i], dw[j][i]))
+      if constexpr (BIAS) GRACE_EACH(db[j][i] += S[j][i])
+      if (g.weight.p != nullptr) {
+        params.get(W, at_lds.at[kW], p);
+        GRACE_EACH(S[j][i] *= p[j][i])
+      }
+      GRACE_EACH(c1 += S[j][i]; c2 = fmaf(S[j][i], hat[j][i], c2))
       sum(c1, c2);
       c1 = n.rms ? 0.f : c1 * inv_d;
       c2 *= inv_d;
@@ -384,8 +529,11 @@ __global__ __launch_bounds__(block_of<TPR>()) void resnorm_bwd_kernel(BwdArgs g)
         row.template store<TX>(g.dx, at, ds);
       }
       if constexpr (GATED) {
-        GRACE_EACH(float u = phat[j][i]; if constexpr (POST) u = u * pw[j][i] + pb[j][i]; u *= S[j][i];
-                   dg[j][i] = g.dgate_mode == kGateRows ? u : dg[j][i] + u; S[j][i] *= gate[j][i])
+        float u[J][V];
+        made_u(u);
+        params.get(G, at_lds.at[kG], p);
+        GRACE_EACH(u[j][i] *= S[j][i]; dg[j][i] = g.dgate_mode == kGateRows ? u[j][i] : dg[j][i] + u[j][i];
+                   S[j][i] *= p[j][i])
         if (g.dgate_mode == kGateRows) {
 #pragma unroll
           for (int j = 0; j < J; ++j)
@@ -394,8 +542,13 @@ __global__ __launch_bounds__(block_of<TPR>()) void resnorm_bwd_kernel(BwdArgs g)
       }
       if constexpr (POST) {
         c1 = c2 = 0.f;
-        GRACE_EACH(dpw[j][i] = fmaf(S[j][i], phat[j][i], dpw[j][i]); dpb[j][i] += S[j][i]; S[j][i] *= pw[j][i];
-                   c1 += S[j][i]; c2 = fmaf(S[j][i], phat[j][i], c2))
+        GRACE_EACH(dpw[j][i] = fmaf(S[j][i], phat[j][i], dpw[j][i]))
+        if constexpr (BIAS) GRACE_EACH(dpb[j][i] += S[j][i])
+        if (g.post_weight.p != nullptr) {
+          params.get(PW, at_lds.at[kPw], p);
+          GRACE_EACH(S[j][i] *= p[j][i])
+        }
+        GRACE_EACH(c1 += S[j][i]; c2 = fmaf(S[j][i], phat[j][i], c2))
         sum(c1, c2);
         c1 = n.rms ? 0.f : c1 * inv_d;
         c2 *= inv_d;
@@ -419,11 +572,11 @@ __global__ __launch_bounds__(block_of<TPR>()) void resnorm_bwd_kernel(BwdArgs g)
     over_slots(acc, row, red, [&](int c, const float(&v)[V], int k) { store_vec(to + c, v, k); });
   };
   leave(kDw, dw);
-  leave(kDb, db);
+  if constexpr (BIAS) leave(kDb, db);
   if constexpr (GATED) leave(kDg, dg);
   if constexpr (POST) {
     leave(kDpw, dpw);
-    leave(kDpb, dpb);
+    if constexpr (BIAS) leave(kDpb, dpb);
   }
 }
 
@@ -440,31 +593,81 @@ void by_width(int d, F&& f) {
   else f(integral_constant<int, 16>{}, integral_constant<int, 1024>{});
 }
 
+// More than 64 KB of dynamic LDS has to be asked for, once for each kernel and device.
+template <auto Kernel>
+void allow_lds(unsigned bytes) {
+  if (bytes <= 60 * 1024) return;
+  static std::atomic<uint64_t> done{0};
+  int dev = 0;
+  if (hipGetDevice(&dev) != hipSuccess || dev > 63) dev = 63;
+  if (done.load(std::memory_order_relaxed) >> dev & 1) return;
+  if (hipFuncSetAttribute(reinterpret_cast<const void*>(Kernel), hipFuncAttributeMaxDynamicSharedMemorySize,
+                          140 * 1024) == hipSuccess && dev < 63)
+    done.fetch_or(1ull << dev, std::memory_order_relaxed);
+}
+
+// Workgroups of a kernel that the chip holds at a time.
+template <auto Kernel>
+unsigned resident(int block, unsigned lds) {
+  static std::atomic<uint64_t> last{0};  // lds + 1 in the upper half, the answer in the lower
+  const uint64_t key = (uint64_t)lds + 1, known = last.load(std::memory_order_relaxed);
+  if (known >> 32 == key) return (unsigned)known;
+  int per_cu = 0;
+  if (hipOccupancyMaxActiveBlocksPerMultiprocessor(&per_cu, Kernel, block, lds) != hipSuccess || per_cu < 1) {
+    (void)hipGetLastError();
+    per_cu = 1;
+  }
+  const unsigned n = (unsigned)per_cu * kCUs;
+  last.store(key << 32 | n, std::memory_order_relaxed);
+  return n;
+}
+
 template <typename TX, typename TY>
-void launch_forward(const FwdArgs& a, unsigned max_blocks, hipStream_t stream) {
+void launch_forward(const FwdArgs& a, hipStream_t stream) {
   by_width(a.n.d, [&](auto e, auto tpr) {
     constexpr int E = decltype(e)::value, TPR = decltype(tpr)::value, B = block_of<TPR>();
-    const unsigned grid = (unsigned)std::min<int64_t>((a.n.rows + B / TPR - 1) / (B / TPR), max_blocks);
-    resnorm_fwd_kernel<TX, TY, E, TPR><<<grid, B, 0, stream>>>(a);
+    const ParamPlaces places(a.weight.p, a.bias.p, a.gate.p, a.n.post ? a.post_weight.p : nullptr,
+                             a.n.post ? a.post_bias.p : nullptr);
+    constexpr int V = vec_of<TX, TY>();
+    const unsigned lds = places.n * Params<1, TPR, V, E / V, lds_forward<E, TPR>()>::kFloats * 4;
+    allow_lds<resnorm_fwd_kernel<TX, TY, E, TPR>>(lds);
+    // a last, half-empty round of workgroups would cost as much as a full one
+    const unsigned grid = (unsigned)std::min<int64_t>((a.n.rows + B / TPR - 1) / (B / TPR),
+                                                      resident<resnorm_fwd_kernel<TX, TY, E, TPR>>(B, lds));
+    resnorm_fwd_kernel<TX, TY, E, TPR><<<grid, B, lds, stream>>>(a);
   });
 }
 
 template <typename TX, typename TY>
 void launch_backward(const BwdArgs& a, hipStream_t stream) {
-  const bool post = a.n.post, gated = a.gate.p != nullptr;
-  by_width(a.n.d, [&](auto e, auto tpr) {
-    constexpr int E = decltype(e)::value, TPR = decltype(tpr)::value, B = block_of<TPR>();
-    const unsigned grid = (unsigned)a.split.blocks;
-    if (post && gated) resnorm_bwd_kernel<TX, TY, E, TPR, true, true><<<grid, B, 0, stream>>>(a);
-    else if (post) resnorm_bwd_kernel<TX, TY, E, TPR, true, false><<<grid, B, 0, stream>>>(a);
-    else if (gated) resnorm_bwd_kernel<TX, TY, E, TPR, false, true><<<grid, B, 0, stream>>>(a);
-    else resnorm_bwd_kernel<TX, TY, E, TPR, false, false><<<grid, B, 0, stream>>>(a);
-  });
+  const bool bias = a.want[kDb] || a.want[kDpb] || a.post_bias.p != nullptr;
+  auto choose = [&](auto post, auto gated, auto biased) {
+    constexpr bool POST = decltype(post)::value, GATED = decltype(gated)::value, BIAS = decltype(biased)::value;
+    by_width(a.n.d, [&](auto e, auto tpr) {
+      constexpr int E = decltype(e)::value, TPR = decltype(tpr)::value, V = vec_of<TX, TY>();
+      const ParamPlaces places(a.weight.p, nullptr, a.gate.p, POST ? a.post_weight.p : nullptr,
+                               POST && BIAS ? a.post_bias.p : nullptr);
+      const unsigned lds = places.n * Params<1, TPR, V, E / V, lds_backward<E, TPR>()>::kFloats * 4;
+      allow_lds<resnorm_bwd_kernel<TX, TY, E, TPR, POST, GATED, BIAS>>(lds);
+      resnorm_bwd_kernel<TX, TY, E, TPR, POST, GATED, BIAS>
+          <<<(unsigned)a.split.blocks, block_of<TPR>(), lds, stream>>>(a);
+    });
+  };
+  auto by_bias = [&](auto post, auto gated) {
+    if (bias) choose(post, gated, std::true_type{});
+    else choose(post, gated, std::false_type{});
+  };
+  auto by_gate = [&](auto post) {
+    if (a.gate.p != nullptr) by_bias(post, std::true_type{});
+    else by_bias(post, std::false_type{});
+  };
+  if (a.n.post) by_gate(std::true_type{});
+  else by_gate(std::false_type{});
 }
 
-// one translation unit per block type (resnorm_f32.hip, resnorm_bf16.hip, resnorm_f16.hip)
+// one translation unit per pair of types (resnorm_*.hip)
 #define GRACE_RESNORM_DECLARE(prefix, TX, TY)                                             \
-  prefix template void launch_forward<TX, TY>(const FwdArgs&, unsigned, hipStream_t);     \
+  prefix template void launch_forward<TX, TY>(const FwdArgs&, hipStream_t);     \
   prefix template void launch_backward<TX, TY>(const BwdArgs&, hipStream_t);
 
 }  // namespace resnorm

@@ -4,6 +4,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 namespace grace {
 
 using bf16_t = __bf16;    // gfx950 converts with v_cvt_pk_bf16_f32 (round to nearest even, NaN kept)
@@ -21,6 +23,56 @@ struct __attribute__((packed, aligned(sizeof(T)))) Pack {
   T v[V];
 };
 
+// The same address, as a value of its own.  The element-wise branch of a partial vector works on it: seeing
+// one address in both branches, the compiler takes the elements they share out of the wide access, which
+// then falls apart into a halfword, two dwords and so on.
+template <typename T>
+__device__ __forceinline__ T* apart(T* p) {
+  asm("" : "+v"(p));
+  return p;
+}
+
+// V elements as stored, in whole registers (two 16-bit values to a register: a struct of elements that
+// lives across a loop gets a register for each)
+template <typename T, int V>
+struct Bits {
+  static constexpr int W = V * (int)sizeof(T) / 4;
+  uint32_t w[W];
+};
+template <int W, int A>
+struct __attribute__((packed, aligned(A))) Words {
+  uint32_t w[W];
+};
+
+// the first n of V elements at p; the others are zero
+template <typename T, int V>
+__device__ __forceinline__ void load_bits(const T* __restrict__ p, Bits<T, V>& o, int n) {
+  constexpr int W = Bits<T, V>::W;
+  if (n >= V) {
+    const Words<W, sizeof(T)> r = *reinterpret_cast<const Words<W, sizeof(T)>*>(p);
+#pragma unroll
+    for (int i = 0; i < W; ++i) o.w[i] = r.w[i];
+  } else {
+#pragma unroll
+    for (int i = 0; i < W; ++i) o.w[i] = 0;
+    const T* q = apart(p);
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      if (i >= n) continue;
+      if constexpr (sizeof(T) == 4) o.w[i] = reinterpret_cast<const uint32_t*>(q)[i];
+      else o.w[i / 2] |= (uint32_t) reinterpret_cast<const uint16_t*>(q)[i] << (16 * (i & 1));
+    }
+  }
+}
+
+template <typename T, int V>
+__device__ __forceinline__ float bits_at(const Bits<T, V>& b, int i) {
+  if constexpr (sizeof(T) == 4) return __uint_as_float(b.w[i]);
+  else if constexpr (std::is_same<T, bf16_t>::value)
+    return __uint_as_float(i & 1 ? b.w[i / 2] & 0xffff0000u : b.w[i / 2] << 16);
+  else return (float)__builtin_bit_cast(half_t, (uint16_t)(b.w[i / 2] >> (16 * (i & 1))));
+}
+
 // the first n of V elements at p, widened to fp32; the others are zero
 template <int V, typename T>
 __device__ __forceinline__ void load_vec(const T* __restrict__ p, float (&o)[V], int n = V) {
@@ -29,8 +81,9 @@ __device__ __forceinline__ void load_vec(const T* __restrict__ p, float (&o)[V],
 #pragma unroll
     for (int i = 0; i < V; ++i) o[i] = (float)r.v[i];
   } else {
+    const T* q = apart(p);
 #pragma unroll
-    for (int i = 0; i < V; ++i) o[i] = i < n ? (float)p[i] : 0.f;
+    for (int i = 0; i < V; ++i) o[i] = i < n ? (float)q[i] : 0.f;
   }
 }
 
@@ -43,9 +96,10 @@ __device__ __forceinline__ void store_vec(T* __restrict__ p, const float (&x)[V]
     for (int i = 0; i < V; ++i) r.v[i] = (T)x[i];
     *reinterpret_cast<Pack<T, V>*>(p) = r;
   } else {
+    T* q = apart(p);
 #pragma unroll
     for (int i = 0; i < V; ++i)
-      if (i < n) p[i] = (T)x[i];
+      if (i < n) q[i] = (T)x[i];
   }
 }
 

@@ -15,8 +15,7 @@ namespace {
 
 using namespace resnorm;
 
-constexpr int kCUs = 256;
-constexpr int kMinRows = 4;  // rows per row slot of a workgroup before another workgroup is added
+constexpr int kMinRows = 2;  // rows per row slot of a workgroup before another workgroup is added
 
 struct FoldArgs {
   const float* part;
@@ -29,26 +28,50 @@ struct FoldArgs {
   int64_t rows[kSums];  // output rows (more than one: dgate's groups)
 };
 
-// One workgroup adds 64 columns of one output row: 16 waves take every 16th partial row each.
+// One workgroup adds 64 columns of one output row.  16 lanes read the columns of a partial row, so the
+// workgroup's 64 slices have 64 x kAhead rows in flight: the launch is one or two latencies long.
+constexpr int kFoldCols = 64, kFoldSlices = 64, kAhead = 4;
 template <typename TY>
 __global__ __launch_bounds__(1024) void resnorm_fold_kernel(FoldArgs a) {
   int64_t row = blockIdx.y;
   int k = 0;
   while (k + 1 < a.sums && row >= a.rows[k]) row -= a.rows[k++];
   const int64_t per = a.blocks / a.rows[k];
-  const int c = blockIdx.x * kWave + lane_id();
-  float v = 0.f;
-  if (c < a.d) {
+  const int slice = threadIdx.x / 16, lane = threadIdx.x % 16;
+  const int c = blockIdx.x * kFoldCols + lane * 4, left = min(a.d - c, 4);
+  float v[4] = {};
+  if (left > 0) {
     const float* p = a.part + ((int64_t)a.which[k] * a.blocks + row * per) * a.d + c;
-    for (int64_t i = wave_id(); i < per; i += 16) v += p[i * a.d];
+    for (int64_t i = slice; i < per; i += kFoldSlices * kAhead) {
+      float x[kAhead][4];
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) x[u][q] = 0.f;
+        if (i + u * kFoldSlices < per) load_vec(p + (i + u * kFoldSlices) * a.d, x[u], left);
+      }
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) v[q] += x[u][q];
+    }
   }
-  __shared__ float red[16][kWave];
-  red[wave_id()][lane_id()] = v;
+  __shared__ float red[kFoldSlices][kFoldCols];
+#pragma unroll
+  for (int q = 0; q < 4; ++q) red[slice][lane * 4 + q] = v[q];
+  // 16 waves: 16 sums of 4 slices, then the first wave joins those
+  const int col = lane_id(), w = wave_id();
   __syncthreads();
-  if (wave_id() == 0 && c < a.d) {
-    for (int i = 1; i < 16; ++i) v += red[i][lane_id()];
-    const float o[1] = {v};
-    store_param<TY>(a.out[k], a.f32[k], row * a.d + c, o, 1);
+  float s = red[4 * w][col] + red[4 * w + 1][col] + red[4 * w + 2][col] + red[4 * w + 3][col];
+  __syncthreads();
+  red[w][col] = s;
+  __syncthreads();
+  const int at = blockIdx.x * kFoldCols + col;
+  if (w == 0 && at < a.d) {
+#pragma unroll
+    for (int i = 1; i < 16; ++i) s += red[i][col];
+    const float o[1] = {s};
+    store_param<TY>(a.out[k], a.f32[k], row * a.d + at, o, 1);
   }
 }
 
@@ -99,7 +122,7 @@ void resnorm_forward(const NormShape& n, const void* x, const void* y, NormParam
   by_types(n, [&](auto* tag_x, auto* tag_y) {
     using TX = std::remove_pointer_t<decltype(tag_x)>;
     using TY = std::remove_pointer_t<decltype(tag_y)>;
-    launch_forward<TX, TY>(a, 2 * shape_of(n.d).resident, stream);
+    launch_forward<TX, TY>(a, stream);
   });
 }
 

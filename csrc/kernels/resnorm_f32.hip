@@ -1,4 +1,4 @@
-// The residual-norm kernels (grace_resnorm.h) for blocks of type f32.
+// The residual-norm kernels (grace_resnorm.h) for a residual of type float and a block of type float.
 #include "grace_resnorm.h"
 
 namespace grace {
