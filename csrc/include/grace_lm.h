@@ -22,6 +22,9 @@ struct EmbedIds {
 void embed_forward(const EmbedIds& ids, const void* w, ElType tw, int64_t w_stride, int64_t d, float scale, void* out,
                    ElType to, hipStream_t stream);
 
+// whether embed_backward clears dw itself (16-byte aligned); it expects zeros otherwise
+bool embed_backward_fills(int64_t n);
+
 // bytes of workspace that embed_backward needs
 int64_t embed_backward_ws(int64_t n, int64_t vocab, int64_t d);
 
@@ -78,6 +81,9 @@ int64_t gradnorm_parts(const GradTensor* g, int64_t n);  // partial values that 
 void gradnorm_partial(const GradTensor* g, int64_t n, NormKind kind, double* part, hipStream_t stream);
 // out[0] = norm, out[1] = min(1, max_norm / (norm + 1e-6)), from any number of partial values
 void gradnorm_finish(const double* part, int64_t parts, NormKind kind, float max_norm, float* out, hipStream_t stream);
+// both at once from the partial values: out as above, and g *= out[1]; no tensors: neither
+void grad_clip(const GradTensor* g, int64_t n, const double* part, int64_t parts, NormKind kind, float max_norm,
+               float* out, hipStream_t stream);
 // g *= *factor (a device value); one leaves the memory untouched.  No two tensors may overlap.
 void grad_scale(const GradTensor* g, int64_t n, const float* factor, hipStream_t stream);
 

@@ -70,6 +70,7 @@ struct BwdArgs {
   NormParam gate, weight, post_weight, post_bias;
   void *dx, *dy, *dgate;
   bool dgate_f32;
+  bool once;  // nontemporal stores
   bool want[kSums];
   int dgate_mode;
   float* part;  // [sums][blocks][d]
@@ -160,10 +161,16 @@ struct Row {
     }
   }
   template <typename T>
-  __device__ __forceinline__ void store(void* p, int64_t at, const float (&v)[J][V]) const {
+  __device__ __forceinline__ void store(void* p, int64_t at, const float (&v)[J][V], bool once) const {
+    if (once) {
 #pragma unroll
-    for (int j = 0; j < J; ++j)
-      if (left[j] > 0) store_vec(static_cast<T*>(p) + at + col(j), v[j], left[j]);
+      for (int j = 0; j < J; ++j)
+        if (left[j] > 0) store_vec<true>(static_cast<T*>(p) + at + col(j), v[j], left[j]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < J; ++j)
+        if (left[j] > 0) store_vec(static_cast<T*>(p) + at + col(j), v[j], left[j]);
+    }
   }
   // mean and 1 / deviation of v, which is zero outside the width
   __device__ __forceinline__ void stats(const float (&v)[J][V], bool rms, float eps, RowSum<TPR>& sum, float& mean,
@@ -352,7 +359,7 @@ __global__ __launch_bounds__(block_of<TPR>()) void resnorm_fwd_kernel(FwdArgs g)
     }
     if (g.x != nullptr) GRACE_EACH(u[j][i] = fmaf(n.alpha, x[j][i], u[j][i]))
     row.trim(u);
-    if (g.s != nullptr) row.template store<TX>(g.s, at, u);
+    if (g.s != nullptr) row.template store<TX>(g.s, at, u, false);
     row.stats(u, n.rms, n.eps, sum, mean, rstd);
     if (g.stats != nullptr && row.t == 0) {
       g.stats[r] = mean;
@@ -367,7 +374,7 @@ __global__ __launch_bounds__(block_of<TPR>()) void resnorm_fwd_kernel(FwdArgs g)
       take(kB, g.bias, p);
       GRACE_EACH(u[j][i] += p[j][i])
     }
-    row.template store<TY>(g.h, at, u);
+    row.template store<TY>(g.h, at, u, false);
     if (!more) return;
     r += step;
     if (!AHEAD) fetch(r);
@@ -526,7 +533,7 @@ __global__ __launch_bounds__(block_of<TPR>(), TPR == 512 ? 4 : 1) void resnorm_b
       row.trim(S);
       if (g.dx != nullptr) {
         GRACE_EACH(ds[j][i] = n.alpha * S[j][i])
-        row.template store<TX>(g.dx, at, ds);
+        row.template store<TX>(g.dx, at, ds, g.once);
       }
       if constexpr (GATED) {
         float u[J][V];
@@ -554,7 +561,7 @@ __global__ __launch_bounds__(block_of<TPR>(), TPR == 512 ? 4 : 1) void resnorm_b
         c2 *= inv_d;
         GRACE_EACH(S[j][i] = prstd * (S[j][i] - c1 - phat[j][i] * c2))
       }
-      row.template store<TY>(g.dy, at, S);
+      row.template store<TY>(g.dy, at, S, g.once);
     }
     if constexpr (GATED) {
       if (g.dgate_mode == kGateGroups) {

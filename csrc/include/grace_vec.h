@@ -44,11 +44,17 @@ struct __attribute__((packed, aligned(A))) Words {
   uint32_t w[W];
 };
 
-// the first n of V elements at p; the others are zero
-template <typename T, int V>
+// the first n of V elements at p; the others are zero.  ONCE: data that passes the caches by (nontemporal)
+template <bool ONCE = false, typename T, int V>
 __device__ __forceinline__ void load_bits(const T* __restrict__ p, Bits<T, V>& o, int n) {
   constexpr int W = Bits<T, V>::W;
   if (n >= V) {
+    if constexpr (ONCE) {
+      typedef uint32_t word __attribute__((aligned(2)));
+#pragma unroll
+      for (int i = 0; i < W; ++i) o.w[i] = __builtin_nontemporal_load(reinterpret_cast<const word*>(p) + i);
+      return;
+    }
     const Words<W, sizeof(T)> r = *reinterpret_cast<const Words<W, sizeof(T)>*>(p);
 #pragma unroll
     for (int i = 0; i < W; ++i) o.w[i] = r.w[i];
@@ -88,12 +94,20 @@ __device__ __forceinline__ void load_vec(const T* __restrict__ p, float (&o)[V],
 }
 
 // one rounding to nearest even (none for fp32) of the first n of V elements
-template <int V, typename T>
+template <bool ONCE = false, int V, typename T>
 __device__ __forceinline__ void store_vec(T* __restrict__ p, const float (&x)[V], int n = V) {
   if (n >= V) {
     Pack<T, V> r;
 #pragma unroll
     for (int i = 0; i < V; ++i) r.v[i] = (T)x[i];
+    if constexpr (ONCE) {
+      typedef uint32_t word __attribute__((aligned(2)));
+      const Words<V * sizeof(T) / 4, 4> w = __builtin_bit_cast(Words<V * sizeof(T) / 4, 4>, r);
+#pragma unroll
+      for (int i = 0; i < V * (int)sizeof(T) / 4; ++i)
+        __builtin_nontemporal_store(w.w[i], reinterpret_cast<word*>(p) + i);
+      return;
+    }
     *reinterpret_cast<Pack<T, V>*>(p) = r;
   } else {
     T* q = apart(p);

@@ -67,7 +67,8 @@ Tensor embed_bwd(const Tensor& ids, const Tensor& dy, int64_t vocab, int64_t pad
   const grace::EmbedIds e = embed_ids(ids, vocab, pad);
   DevGuard guard(dy.device());
   const auto tdw = el_type(dtype, "embedding: the table"), tdy = el_type(dy.scalar_type(), "embedding: the gradient");
-  Tensor dw = at::zeros({vocab, d}, dy.options().dtype(dtype));
+  Tensor dw = grace::embed_backward_fills(e.n) ? at::empty({vocab, d}, dy.options().dtype(dtype))
+                                               : at::zeros({vocab, d}, dy.options().dtype(dtype));
   Tensor ws = at::empty({grace::embed_backward_ws(e.n, vocab, d)}, dy.options().dtype(at::kByte));
   grace::embed_backward(e, dy.data_ptr(), tdy, d, (float)scale, dw.data_ptr(), tdw, ws.data_ptr(), cur_stream());
   C10_HIP_KERNEL_LAUNCH_CHECK();
@@ -384,12 +385,13 @@ OptTensor grad_clip(const std::vector<Tensor>& params, int64_t kind, double max_
   if (grads.empty()) return c10::nullopt;
   DevGuard guard(grads[0].device());
   const auto g = grad_list(grads);
-  Tensor out = grad_norm_finish(parts_of(g, norm_kind(kind), grads[0]), kind, max_norm);
-  if (scale) {
-    grace::grad_scale(g.data(), (int64_t)g.size(), out.data_ptr<float>() + 1, cur_stream());
-    C10_HIP_KERNEL_LAUNCH_CHECK();
-    for (const Tensor& t : grads) t.unsafeGetTensorImpl()->bump_version();
-  }
+  const Tensor part = parts_of(g, norm_kind(kind), grads[0]);
+  if (!scale || g.empty()) return grad_norm_finish(part, kind, max_norm);
+  Tensor out = at::empty({2}, grads[0].options().dtype(at::kFloat));
+  grace::grad_clip(g.data(), (int64_t)g.size(), part.data_ptr<double>(), part.numel(), norm_kind(kind),
+                   (float)max_norm, out.data_ptr<float>(), cur_stream());
+  C10_HIP_KERNEL_LAUNCH_CHECK();
+  for (const Tensor& t : grads) t.unsafeGetTensorImpl()->bump_version();
   return out;
 }
 
