@@ -97,6 +97,11 @@ def parse():
     ap.add_argument("--optimizer", choices=["fused", "torch"], default="fused",
                     help="fused: grace_amd FusedSGD (one native multi-tensor kernel that also writes the bf16 "
                          "working copies); torch: torch.optim.SGD (foreach)")
+    ap.add_argument("--lm-ops", choices=["torch", "fused"], default="torch",
+                    help="bert / lstm workloads: fused = the framework's embedding (sorted gradient) and residual "
+                         "norms (ops/embedding.py, ops/norm.py)")
+    ap.add_argument("--max-grad-norm", type=float, default=None,
+                    help="clip by the global gradient norm inside the fused optimizer's update (parallel/clip.py)")
     ap.add_argument("--grad-mode", choices=["gather", "accumulate"], default="gather",
                     help="gather: zero_grad(set_to_none) + one native gather launch per bucket; "
                          "accumulate: bucket memset + AccumulateGrad adds into bucket views")
@@ -277,7 +282,7 @@ def main() -> int:
     w = WORKLOADS[args.workload]
     batch = args.batch or w.batch
     torch.manual_seed(0)
-    model = build_model(w, dev)
+    model = build_model(w, dev, args.lm_ops)
     broadcast_parameters(model.state_dict(), root_rank=0)
     weights = None
     named = list(model.named_parameters())
@@ -289,8 +294,10 @@ def main() -> int:
     if args.optimizer == "fused":
         from grace_amd.parallel import FusedSGD
 
-        base_opt = FusedSGD([p for _, p in named], lr=0.01 * world, momentum=0.5)
+        base_opt = FusedSGD([p for _, p in named], lr=0.01 * world, momentum=0.5, max_grad_norm=args.max_grad_norm)
     else:
+        if args.max_grad_norm is not None:
+            raise SystemExit("--max-grad-norm needs --optimizer fused")
         base_opt = torch.optim.SGD([p for _, p in named], lr=0.01 * world, momentum=0.5)
     from grace_amd.parallel.graph import GraphedStep, graph_compute, graph_safe
 
@@ -706,7 +713,9 @@ def main() -> int:
                 "surface": args.surface + (f" ({len(ddp_state.layouts)} DDP buckets, "
                                            f"{'deferred' if ddp_state.defer else 'immediate'} hook)" if ddp_state else ""),
                 "bf16_weights": weights is not None,
-                "optimizer": f"{'FusedSGD' if args.optimizer == 'fused' else 'torch.optim.SGD'}(lr={0.01 * world:g}, momentum=0.5)",
+                "optimizer": f"{'FusedSGD' if args.optimizer == 'fused' else 'torch.optim.SGD'}(lr={0.01 * world:g}, momentum=0.5"
+                             + (f", max_grad_norm={args.max_grad_norm:g})" if args.max_grad_norm is not None else ")"),
+                **({"lm_ops": args.lm_ops} if args.lm_ops != "torch" else {}),
             },
             "per_gpu": {"mean": round(mean_pg, 2), "ci95": round(1.96 * std_pg, 2),
                         "note": f"{w.unit}/sec per GPU on rank 0, mean +- 1.96 std over {len(per_gpu)} steps"},

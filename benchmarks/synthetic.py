@@ -23,7 +23,8 @@ import torch
 sys.path.insert(0, os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
 
 from grace_amd import grace_from_params  # noqa: E402
-from grace_amd.parallel import DistributedOptimizer, broadcast_optimizer_state, broadcast_parameters  # noqa: E402
+from grace_amd.parallel import (DistributedOptimizer, broadcast_optimizer_state,  # noqa: E402
+                                broadcast_parameters, clip_grad_norm_)
 from grace_amd.parallel.launch import init_distributed  # noqa: E402
 from grace_amd.utils.workloads import WORKLOADS, build_model  # noqa: E402
 
@@ -47,6 +48,10 @@ def main():
     ap.add_argument("--threshold", type=float, default=None)
     ap.add_argument("--efsgd-lr", type=float, default=None)
     ap.add_argument("--bucket-mb", type=float, default=64.0)
+    ap.add_argument("--lm-ops", choices=["torch", "fused"], default="torch",
+                    help="bert / lstm: fused = the framework's embedding and residual norms")
+    ap.add_argument("--max-grad-norm", type=float, default=None,
+                    help="clip the exchanged gradients by their global norm (parallel/clip.py)")
     ap.add_argument("--fp32", action="store_true", help="disable bf16 autocast")
     ap.add_argument("--json", action="store_true")
     a = ap.parse_args()
@@ -63,7 +68,7 @@ def main():
             params[k] = v
     params["world_size"] = world
     torch.backends.cudnn.benchmark = True
-    model = build_model(w, dev)
+    model = build_model(w, dev, a.lm_ops)
     batch = a.batch_size or w.batch
     opt = torch.optim.SGD(model.parameters(), lr=a.lr * world, momentum=a.momentum)
     broadcast_parameters(model.state_dict(), root_rank=0)
@@ -77,7 +82,13 @@ def main():
         with torch.autocast(dev.type, dtype=torch.bfloat16, enabled=not a.fp32 and dev.type == "cuda"):
             loss = w.loss(model, data)
         loss.backward()
-        opt.step()
+        if a.max_grad_norm is None:
+            opt.step()
+        else:
+            opt.synchronize()
+            clip_grad_norm_(model.parameters(), a.max_grad_norm)
+            with opt.skip_synchronize():
+                opt.step()
         if dev.type == "cuda":
             torch.cuda.synchronize()
 

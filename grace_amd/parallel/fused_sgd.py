@@ -79,14 +79,19 @@ class FusedSGD(SGD):
         factor = self._clip_factor() if self.max_grad_norm is not None else None
         for group in self.param_groups:
             native, rest = [], []
+            on = {}  # device -> whether its native path runs
             for p in group["params"]:
-                if p.grad is None:
+                g = p.grad
+                if g is None:
                     continue
-                if p.grad.is_sparse:
+                if g.is_sparse:
                     raise RuntimeError("FusedSGD does not support sparse gradients")
-                ok = (p.is_cuda and _native.native_on(p.device) and p.dtype == torch.float32
-                      and p.grad.dtype == torch.float32 and _same_layout(p.grad, p)
-                      and _dense(p))
+                dev = p.device
+                if dev not in on:
+                    on[dev] = _native.native_on(dev)
+                ok = (on[dev] and p.dtype == torch.float32 and g.dtype == torch.float32
+                      and (p.is_contiguous() and g.is_contiguous() and p.shape == g.shape
+                           or _same_layout(g, p) and _dense(p)))
                 (native if ok else rest).append(p)
             if native:
                 self._native_step(group, native, factor)
@@ -127,7 +132,7 @@ class FusedSGD(SGD):
                 devs.setdefault((p.device, is_first), []).append(p)
         for (dev, is_first), ps in devs.items():
             bufs = [self.state[p].get("momentum_buffer") if mom != 0 else None for p in ps]
-            w16 = [self._working_for(p) for p in ps]
+            w16 = [self._working_for(p) for p in ps] if self._working else [None] * len(ps)
             _native.lib().sgd_step(ps, [p.grad for p in ps], bufs, w16, float(group["lr"]), float(mom),
                                    float(group["dampening"]), float(group["weight_decay"]),
                                    bool(group["nesterov"]), bool(group.get("maximize", False)), is_first,
@@ -137,6 +142,8 @@ class FusedSGD(SGD):
                     self._working[id(p)].copy_(p)
 
     def _working_for(self, p) -> Optional[torch.Tensor]:
+        if not self._working:
+            return None
         w = self._working.get(id(p))
         return w if (w is not None and _same_layout(w, p)) else None
 

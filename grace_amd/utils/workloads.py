@@ -130,8 +130,18 @@ for _k in ("vgg16_powersgd", "lstm_efsignsgd", "bert_qsgd"):
                              _w.seq_len)
 
 
-def build_model(w: Workload, device) -> torch.nn.Module:
-    m = MODELS[w.model](**w.model_kw).to(device)
+LM_MODELS = ("bert_base", "lstm_ptb")  # models with a ``fused`` form (ops/embedding.py, ops/norm.py)
+
+
+def build_model(w: Workload, device, lm_ops: str = "torch") -> torch.nn.Module:
+    kw = dict(w.model_kw)
+    if lm_ops not in ("torch", "fused"):
+        raise ValueError(f"lm_ops {lm_ops!r}: 'torch' or 'fused'")
+    if lm_ops == "fused":
+        if w.model not in LM_MODELS:
+            raise ValueError(f"{w.model} has no fused language-model operators: {', '.join(LM_MODELS)}")
+        kw["fused"] = True
+    m = MODELS[w.model](**kw).to(device)
     if w.channels_last and device.type == "cuda":
         m = m.to(memory_format=torch.channels_last)
     return m
