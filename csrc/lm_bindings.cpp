@@ -34,10 +34,11 @@ void check_on(const Tensor& t, const Tensor& like, const char* what) {
 }
 
 // ---------------------------------------------------------------- embedding
-grace::EmbedIds embed_ids(const Tensor& ids, int64_t vocab, int64_t pad) {
+grace::EmbedIds embed_ids(const Tensor& ids, int64_t vocab, int64_t width, int64_t pad) {
   TORCH_CHECK(ids.is_cuda() && ids.is_contiguous() && (ids.scalar_type() == at::kLong || ids.scalar_type() == at::kInt),
               "embedding: ids must be a contiguous int64 or int32 GPU tensor");
   TORCH_CHECK(ids.numel() < INT32_MAX && vocab < INT32_MAX, "embedding: at most 2^31 - 2 tokens and rows");
+  TORCH_CHECK(width <= grace::kEmbedMaxWidth, "embedding: rows of at most ", grace::kEmbedMaxWidth, " values");
   TORCH_CHECK(pad >= -1 && pad < vocab, "embedding: padding_idx out of range");
   return {ids.data_ptr(), ids.scalar_type() == at::kLong, ids.numel(), vocab, pad};
 }
@@ -47,7 +48,7 @@ Tensor embed_fwd(const Tensor& ids, const Tensor& weight, double scale, at::Scal
               "embedding: the table must be a 2-D GPU tensor with contiguous rows");
   check_on(ids, weight, "embedding: ids");
   TORCH_CHECK(weight.size(0) > 0 || ids.numel() == 0, "embedding: the table has no rows");
-  const grace::EmbedIds e = embed_ids(ids, weight.size(0), -1);
+  const grace::EmbedIds e = embed_ids(ids, weight.size(0), weight.size(1), -1);
   DevGuard guard(weight.device());
   auto shape = ids.sizes().vec();
   shape.push_back(weight.size(1));
@@ -64,7 +65,7 @@ Tensor embed_bwd(const Tensor& ids, const Tensor& dy, int64_t vocab, int64_t pad
   const int64_t d = dy.size(-1);
   TORCH_CHECK(dy.numel() == ids.numel() * d, "embedding: the gradient must be [tokens, width]");
   check_on(ids, dy, "embedding: ids");
-  const grace::EmbedIds e = embed_ids(ids, vocab, pad);
+  const grace::EmbedIds e = embed_ids(ids, vocab, d, pad);
   DevGuard guard(dy.device());
   const auto tdw = el_type(dtype, "embedding: the table"), tdy = el_type(dy.scalar_type(), "embedding: the gradient");
   Tensor dw = grace::embed_backward_fills(e.n) ? at::empty({vocab, d}, dy.options().dtype(dtype))
@@ -79,6 +80,11 @@ Tensor embed_bwd(const Tensor& ids, const Tensor& dy, int64_t vocab, int64_t pad
 // time, where a Python function costs some fifty.  They are differentiable once.
 void once_only(const char* what) {
   TORCH_CHECK(!at::GradMode::is_enabled(), what, " is differentiable once: no create_graph");
+}
+
+// A call that autograd does not follow would lose forward-mode tangents without a word.
+void no_tangent(const Tensor& t, const char* what) {
+  TORCH_CHECK_NOT_IMPLEMENTED(!t._fw_grad(0).defined(), what, " has no forward-mode derivative");
 }
 
 struct EmbeddingFn : torch::autograd::Function<EmbeddingFn> {
@@ -101,6 +107,7 @@ struct EmbeddingFn : torch::autograd::Function<EmbeddingFn> {
 };
 
 Tensor embedding(const Tensor& ids, const Tensor& weight, double scale, int64_t pad, at::ScalarType dtype) {
+  no_tangent(weight, "embedding");
   const Tensor i = ids.contiguous();
   const Tensor w = weight.dim() == 2 && weight.stride(1) != 1 && weight.size(1) > 1 ? weight.contiguous() : weight;
   if (at::GradMode::is_enabled() && w.requires_grad()) return EmbeddingFn::apply(w, i, scale, pad, dtype);
@@ -131,7 +138,7 @@ grace::NormShape norm_shape(const Tensor& y, at::ScalarType tx, int64_t gate_row
   return n;
 }
 
-int64_t gate_size(const grace::NormShape& n) { return n.rows / n.gate_rows * n.d; }
+int64_t gate_size(const grace::NormShape& n) { return n.rows / n.gate_rows * n.d; }  // of rows > 0
 
 struct NormTensors {
   Tensor y, x, gate, weight, bias, post_weight, post_bias;  // undefined: not there
@@ -197,21 +204,21 @@ std::vector<Tensor> resnorm_bwd(const Tensor& dh, const Tensor& ds, const NormTe
   TORCH_CHECK(stats.is_cuda() && stats.scalar_type() == at::kFloat && stats.is_contiguous() &&
                   stats.numel() == (o.post ? 4 : 2) * n.rows, "residual norm: the saved statistics");
   DevGuard guard(like.device());
-  const grace::NormParam gp = norm_param(t.gate, gate_size(n), shape, "residual norm: the gate");
-  const grace::NormParam wp = norm_param(t.weight, n.d, shape, "residual norm: weight");
-  const grace::NormParam bp = norm_param(t.bias, n.d, shape, "residual norm: bias");
-  const grace::NormParam pwp = norm_param(t.post_weight, n.d, shape, "residual norm: post_weight");
-  const grace::NormParam pbp = norm_param(t.post_bias, n.d, shape, "residual norm: post_bias");
   auto made = [&](int k, const Tensor& p) {
     if (!want[k] || !p.defined()) return Tensor();
     return n.rows > 0 ? at::empty_like(p) : at::zeros_like(p);
   };
   Tensor dy = at::empty_like(shape);
-  const bool one = !gp.p && !o.post && n.alpha == 1.f && n.tx == n.ty;
+  const bool one = !t.gate.defined() && !o.post && n.alpha == 1.f && n.tx == n.ty;
   Tensor dx = !want[1] ? Tensor() : one ? dy : at::empty(like.sizes(), like.options().dtype(tx));
   Tensor dgate = made(2, t.gate), dw = made(3, t.weight), db = made(4, t.bias), dpw = made(5, t.post_weight),
          dpb = made(6, t.post_bias);
   if (n.rows > 0) {
+    const grace::NormParam gp = norm_param(t.gate, gate_size(n), shape, "residual norm: the gate");
+    const grace::NormParam wp = norm_param(t.weight, n.d, shape, "residual norm: weight");
+    const grace::NormParam bp = norm_param(t.bias, n.d, shape, "residual norm: bias");
+    const grace::NormParam pwp = norm_param(t.post_weight, n.d, shape, "residual norm: post_weight");
+    const grace::NormParam pbp = norm_param(t.post_bias, n.d, shape, "residual norm: post_bias");
     auto ptr = [](const Tensor& u) { return u.defined() ? u.data_ptr() : nullptr; };
     const grace::NormGrads g{ptr(dx), dy.data_ptr(), ptr(dgate), ptr(dw), ptr(db), ptr(dpw), ptr(dpb), bp.f32, pbp.f32};
     Tensor ws = at::empty({grace::resnorm_backward_ws(n)}, like.options().dtype(at::kByte));
@@ -276,10 +283,13 @@ std::vector<Tensor> residual_norm(const Tensor& y, const OptTensor& x, const Opt
   auto get = [](const OptTensor& t) { return has(t) ? t->contiguous() : Tensor(); };
   const NormTensors t{y.contiguous(), get(x), get(gate), get(weight), get(bias), get(post_weight), get(post_bias)};
   const NormOptions o{gate_rows, post, rms, alpha, eps};
+  const bool follow = at::GradMode::is_enabled();
   bool grad = false;
-  if (at::GradMode::is_enabled())
-    for (const Tensor* p : {&t.y, &t.x, &t.gate, &t.weight, &t.bias, &t.post_weight, &t.post_bias})
-      grad |= p->defined() && p->requires_grad();
+  for (const Tensor* p : {&t.y, &t.x, &t.gate, &t.weight, &t.bias, &t.post_weight, &t.post_bias}) {
+    if (!p->defined()) continue;
+    no_tangent(*p, "residual norm");
+    grad |= follow && p->requires_grad();
+  }
   if (grad) {
     auto opt = [](const Tensor& u) { return u.defined() ? OptTensor(u) : OptTensor(); };
     return ResidualNormFn::apply(t.y, opt(t.x), opt(t.gate), opt(t.weight), opt(t.bias), opt(t.post_weight),
@@ -405,6 +415,7 @@ void grace_bind_lm(py::module& m) {
   m.def("embedding", [](const Tensor& ids, const Tensor& weight, double scale, int64_t pad, const py::object& dtype) {
     return embedding(ids, weight, scale, pad, scalar_type(dtype));
   });
+  m.attr("embed_max_width") = (int64_t)grace::kEmbedMaxWidth;
   m.attr("resnorm_max_width") = (int64_t)grace::kNormMaxWidth;
   m.def("residual_norm", &residual_norm);
   m.def("grad_norm_parts", &grad_norm_parts);

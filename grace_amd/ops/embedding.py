@@ -49,6 +49,8 @@ def embedding(ids: torch.Tensor, weight: torch.Tensor, scale: float = 1.0, paddi
             raise TypeError(f"embedding: float32, bfloat16 or float16 on a GPU, got {weight.dtype} -> {dtype}")
         if ids.numel() >= 2**31 - 1 or rows >= 2**31 - 1:
             raise ValueError("embedding: at most 2^31 - 2 tokens and rows")
+        if weight.shape[1] > _native.lib().embed_max_width:
+            raise ValueError(f"embedding: rows of {weight.shape[1]} values: at most {_native.lib().embed_max_width}")
         return _native.lib().embedding(ids, weight, float(scale), pad, dtype)
     wide = weight if weight.dtype == torch.float64 else weight.float()
     return (F.embedding(ids, wide, None if pad < 0 else pad) * float(scale)).to(dtype)

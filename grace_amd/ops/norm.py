@@ -113,6 +113,8 @@ def residual_norm(y: torch.Tensor, residual: Optional[torch.Tensor] = None, weig
         return (h, y if plain else s.to(y.dtype if residual is None else residual.dtype)) if return_sum else h
     if width > _native.lib().resnorm_max_width:
         raise ValueError(f"residual_norm: a width of {width}: at most {_native.lib().resnorm_max_width} on a GPU")
+    if y.numel() // width >= 2**31 - 1:
+        raise ValueError("residual_norm: at most 2^31 - 2 rows")
     out = _native.lib().residual_norm(y, residual, gate, gate_rows, weight, bias, post_weight, post_bias, post, rms,
                                       alpha, eps, return_sum)
     return tuple(out) if return_sum else out[0]

@@ -140,6 +140,8 @@ def clip_grad_norm_(parameters: Union[torch.Tensor, Iterable[torch.Tensor]], max
     norm makes the gradients NaN or zero, as torch's function does; ``error_if_nonfinite`` raises instead,
     before anything is scaled, for which it waits for the device."""
     kind, max_norm = _kind(norm_type), float(max_norm)
+    if not max_norm >= 0:
+        raise ValueError(f"max_norm {max_norm}: not negative")
     parameters = [parameters] if isinstance(parameters, torch.Tensor) else list(parameters)
     if not error_if_nonfinite and parameters and _native.use_native(parameters[0]):
         out = _native.lib().grad_clip(parameters, kind, max_norm, True)

@@ -44,6 +44,9 @@ def _same_layout(a: torch.Tensor, b: torch.Tensor) -> bool:
 
 
 class FusedSGD(SGD):
+    max_grad_norm: Optional[float] = None
+    grad_norm: Optional[torch.Tensor] = None
+
     def __init__(self, params, lr=1e-3, momentum=0.0, dampening=0.0, weight_decay=0.0, nesterov=False, *,
                  maximize: bool = False, max_grad_norm: Optional[float] = None):
         if max_grad_norm is not None and not max_grad_norm >= 0:
@@ -52,7 +55,6 @@ class FusedSGD(SGD):
                          nesterov=nesterov, maximize=maximize)
         self._working: Dict[int, torch.Tensor] = {}
         self.max_grad_norm = max_grad_norm
-        self.grad_norm: Optional[torch.Tensor] = None
         # the kernel honours the process-wide communication fault flag (parallel/health.py):
         # allocate it now, before any HIP-graph capture of the step
         devs = {p.device for g in self.param_groups for p in g["params"] if p.is_cuda}

@@ -190,6 +190,69 @@ def test_residual_norm_special_values():
         residual_norm(torch.zeros(1, 4, device="cuda", dtype=F64))
 
 
+@pytest.mark.parametrize("tx,ty", [(F32, F32), (BF16, BF16), (F32, F16)])
+def test_residual_norm_empty_batch(tx, ty):
+    for gate in ("none", "sample", "full", "channel"):
+        v, dh, ds = norm_inputs(0, 3, 20, tx, ty, gate, True, True, "cuda")
+        leaves = {k: t.requires_grad_() for k, t in v.items() if t is not None}
+        h, s = residual_norm(v["y"], v["x"], v["weight"], v["bias"], gate=v["gate"], post=True,
+                             post_weight=v["post_weight"], post_bias=v["post_bias"], return_sum=True)
+        assert h.shape == s.shape == (0, 3, 20)
+        for g, p in zip(torch.autograd.grad([h, s], list(leaves.values()), [dh, ds]), leaves.values()):
+            assert g.shape == p.shape and not g.any()
+
+
+@pytest.mark.parametrize("weight,bias", [(False, False), (False, True), (True, False)])
+@pytest.mark.parametrize("post", [False, True])
+def test_residual_norm_without_weights(weight, bias, post):
+    v, dh, ds = norm_inputs(3, 5, 200, BF16, BF16, "none", post, True, "cuda")
+    for on, names in ((weight, ("weight", "post_weight")), (bias, ("bias", "post_bias"))):
+        for n in names:
+            v[n] = v[n] if on else None
+    norm_case(v, dh, ds, "layer", 1.0, post)
+
+
+def test_residual_norm_of_a_sum_with_itself():
+    y = torch.randn(7, 90, device="cuda", requires_grad=True)
+    dh = torch.randn(7, 90, device="cuda")
+    got, = torch.autograd.grad(residual_norm(y, y), y, dh)
+    z = y.detach().requires_grad_()
+    a, = torch.autograd.grad(residual_norm(z, y.detach()), z, dh)
+    # both ways into the sum carry the same gradient: their fp32 sum is exact
+    assert torch.equal(got, a + a)
+    y.grad = None
+    residual_norm(y, y).backward(dh)
+    assert torch.equal(y.grad, a + a)
+
+
+def test_differentiable_once():
+    w = torch.randn(30, 8, device="cuda", requires_grad=True)
+    ids = torch.randint(0, 30, (5,), device="cuda")
+    for f in (lambda: embedding(ids, w), lambda: residual_norm(w)):
+        out = f()
+        with pytest.raises(RuntimeError):
+            torch.autograd.grad(out.sum(), w, create_graph=True)
+        with torch.autograd.forward_ad.dual_level():
+            dual = torch.autograd.forward_ad.make_dual(w.detach(), torch.ones_like(w))
+            with pytest.raises((RuntimeError, NotImplementedError)):
+                embedding(ids, dual)
+            with pytest.raises((RuntimeError, NotImplementedError)):
+                residual_norm(dual)
+    y = w.detach().clone().requires_grad_()
+    h = residual_norm(y * 1.0, w)
+    with torch.no_grad():
+        w.add_(1.0)
+    got, = torch.autograd.grad(h.sum(), y)  # fp32 keeps the sum, not its parts
+    assert torch.isfinite(got).all()
+    x = w.detach().bfloat16().requires_grad_()
+    z = x * 1.0
+    h = residual_norm(z, x)
+    with torch.no_grad():
+        z.add_(1.0)  # a saved tensor has changed
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(h.sum(), x)
+
+
 def test_residual_norm_far_rows():
     """More than 2^31 elements: the last rows are where they belong."""
     y = torch.zeros(2**20 + 3, 2100, dtype=BF16, device="cuda")
@@ -369,6 +432,31 @@ def test_operators_on_another_stream():
             got.append(run())
     torch.cuda.synchronize()
     for outs in got:
+        for a, e in zip(outs, want):
+            assert torch.equal(a, e)
+
+
+def test_wide_rows_in_a_graph():
+    """The widest LDS use, and a graph as the first call of its kernels."""
+    v, dh, ds = norm_inputs(2, 40, 3000, BF16, BF16, "sample", True, True, "cuda")
+
+    def run():
+        t = {k: p.detach().requires_grad_() for k, p in v.items()}
+        h, s = residual_norm(t["y"], t["x"], t["weight"], t["bias"], gate=t["gate"], post=True,
+                             post_weight=t["post_weight"], post_bias=t["post_bias"], return_sum=True)
+        return [h.detach(), s.detach(), *torch.autograd.grad([h, s], list(t.values()), [dh, ds])]
+
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = run()
+    for _ in range(3):
+        with torch.no_grad():
+            v["y"].mul_(1.25)
+        want = run()
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
         for a, e in zip(outs, want):
             assert torch.equal(a, e)
 

@@ -240,6 +240,9 @@ def test_clip_refusals():
     for p in (0.0, 3.0, -math.inf):
         with pytest.raises(ValueError):
             clip_grad_norm_(ps, 1.0, p)
+    for bound in (-1.0, math.nan):
+        with pytest.raises(ValueError):
+            clip_grad_norm_(ps, bound)
     q = nn.Parameter(torch.zeros(3, 4))
     q.grad = torch.ones(1, 4).expand(3, 4)
     with pytest.raises(ValueError):
