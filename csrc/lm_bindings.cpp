@@ -106,10 +106,32 @@ struct EmbeddingFn : torch::autograd::Function<EmbeddingFn> {
   }
 };
 
-Tensor embedding(const Tensor& ids, const Tensor& weight, double scale, int64_t pad, at::ScalarType dtype) {
+Tensor embedding(const Tensor& ids, const Tensor& weight, double scale, const c10::optional<int64_t>& padding_idx,
+                 const c10::optional<at::ScalarType>& out) {
+  auto refuse = [](const std::string& what) { return "embedding: " + what; };
+  const auto tw = weight.scalar_type(), dtype = out.value_or(tw);
+  if (ids.scalar_type() != at::kLong && ids.scalar_type() != at::kInt)
+    throw py::type_error(refuse(c10::str("ids must be int64 or int32, got ", ids.scalar_type())));
+  if (weight.dim() != 2) throw py::value_error(refuse(c10::str("the table must be [rows, width], got ", weight.sizes())));
+  if (ids.device() != weight.device())
+    throw py::value_error(refuse(c10::str("ids on ", ids.device(), ", table on ", weight.device())));
+  const int64_t rows = weight.size(0);
+  if (rows == 0 && ids.numel() > 0) throw py::value_error(refuse("the table has no rows"));
+  int64_t pad = -1;
+  if (padding_idx.has_value()) {
+    pad = *padding_idx < 0 ? *padding_idx + rows : *padding_idx;
+    if (pad < 0 || pad >= rows)
+      throw py::value_error(refuse(c10::str("padding_idx ", *padding_idx, " outside a table of ", rows, " rows")));
+  }
+  for (const auto t : {tw, dtype})
+    if (t != at::kFloat && t != at::kBFloat16 && t != at::kHalf)
+      throw py::type_error(refuse(c10::str("float32, bfloat16 or float16 on a GPU, got ", tw, " -> ", dtype)));
+  if (ids.numel() >= INT32_MAX || rows >= INT32_MAX) throw py::value_error(refuse("at most 2^31 - 2 tokens and rows"));
+  if (weight.size(1) > grace::kEmbedMaxWidth)
+    throw py::value_error(refuse(c10::str("rows of ", weight.size(1), " values: at most ", grace::kEmbedMaxWidth)));
   no_tangent(weight, "embedding");
   const Tensor i = ids.contiguous();
-  const Tensor w = weight.dim() == 2 && weight.stride(1) != 1 && weight.size(1) > 1 ? weight.contiguous() : weight;
+  const Tensor w = weight.stride(1) != 1 && weight.size(1) > 1 ? weight.contiguous() : weight;
   if (at::GradMode::is_enabled() && w.requires_grad()) return EmbeddingFn::apply(w, i, scale, pad, dtype);
   return embed_fwd(i, w, scale, dtype);
 }
@@ -275,13 +297,73 @@ struct ResidualNormFn : torch::autograd::Function<ResidualNormFn> {
   }
 };
 
+// Consecutive rows of y that share one row of the gate, or -1: the gate is [width], or of y's shape with 1 in
+// place of trailing dimensions before the last.
+int64_t gate_rows_of(const Tensor& gate, const Tensor& y) {
+  const int64_t lead = y.dim() - 1;
+  if (gate.size(-1) != y.size(-1) || (gate.dim() != 1 && gate.dim() != y.dim())) return -1;
+  auto size = [&](int64_t k) { return gate.dim() == y.dim() ? gate.size(k) : 1; };
+  int64_t k = 0, rows = 1;
+  while (k < lead && size(k) == y.size(k)) ++k;
+  for (; k < lead; ++k) {
+    if (size(k) != 1) return -1;
+    rows *= y.size(k);
+  }
+  return rows;
+}
+
+// The same refusals, by value and by type, as the Python form of the operator makes for CPU tensors.
+template <typename Error, typename... A>
+void refuse_if(bool bad, const A&... what) {
+  if (C10_UNLIKELY(bad)) throw Error(c10::str("residual_norm: ", what...));
+}
+
 // h, and s with return_sum
-std::vector<Tensor> residual_norm(const Tensor& y, const OptTensor& x, const OptTensor& gate, int64_t gate_rows,
-                                  const OptTensor& weight, const OptTensor& bias, const OptTensor& post_weight,
-                                  const OptTensor& post_bias, bool post, bool rms, double alpha, double eps,
-                                  bool return_sum) {
-  auto get = [](const OptTensor& t) { return has(t) ? t->contiguous() : Tensor(); };
-  const NormTensors t{y.contiguous(), get(x), get(gate), get(weight), get(bias), get(post_weight), get(post_bias)};
+std::vector<Tensor> residual_norm(const Tensor& y, const OptTensor& x, const OptTensor& weight, const OptTensor& bias,
+                                  const std::string& kind, double eps, const OptTensor& gate, double alpha, bool post,
+                                  const OptTensor& post_weight, const OptTensor& post_bias, bool return_sum) {
+  const bool rms = kind == "rms";
+  using Value = py::value_error;
+  using Type = py::type_error;
+  refuse_if<Value>(!rms && kind != "layer", "kind '", kind, "': 'layer' or 'rms'");
+  refuse_if<Value>(y.dim() < 1 || y.size(-1) < 1, "a block of shape ", y.sizes());
+  refuse_if<Value>(!post && (has(post_weight) || has(post_bias)), "post_weight and post_bias need post=True");
+  const auto ty = y.scalar_type();
+  refuse_if<Type>(ty != at::kFloat && ty != at::kBFloat16 && ty != at::kHalf, "a block of ", ty);
+  const int64_t width = y.size(-1);
+  if (has(x)) {
+    refuse_if<Value>(x->sizes() != y.sizes() || x->device() != y.device(), "a residual of ", x->sizes(), " on ",
+                     x->device(), " for a block of ", y.sizes(), " on ", y.device());
+    refuse_if<Type>(x->scalar_type() != ty && x->scalar_type() != at::kFloat, "a residual of ", x->scalar_type(),
+                    " for a block of ", ty);
+  } else {
+    refuse_if<Value>(alpha != 1.0, "alpha scales a residual, and there is none");
+  }
+  auto param = [&](const OptTensor& p, const char* name, bool shaped) {
+    if (!has(p)) return Tensor();
+    refuse_if<Value>(p->device() != y.device(), name, " on ", p->device(), ", the block on ", y.device());
+    refuse_if<Type>(p->scalar_type() != ty && p->scalar_type() != at::kFloat, name, " of ", p->scalar_type(),
+                    " for a block of ", ty);
+    refuse_if<Value>(shaped && (p->dim() != 1 || p->size(0) != width), name, " of shape ", p->sizes(), " for a width of ",
+                     width);
+    return p->contiguous();
+  };
+  const NormTensors t{y.contiguous(),
+                      has(x) ? x->contiguous() : Tensor(),
+                      param(gate, "gate", false),
+                      param(weight, "weight", true),
+                      param(bias, "bias", true),
+                      param(post_weight, "post_weight", true),
+                      param(post_bias, "post_bias", true)};
+  const int64_t rows = y.numel() / width;
+  int64_t gate_rows = rows;
+  if (t.gate.defined()) {
+    gate_rows = t.gate.dim() < 1 ? -1 : gate_rows_of(t.gate, y);
+    refuse_if<Value>(gate_rows < 0, "a gate of shape ", t.gate.sizes(), " for a block of ", y.sizes(),
+                     ": it is [width], or the block's shape with 1 in place of trailing dimensions before the last");
+  }
+  refuse_if<Value>(width > grace::kNormMaxWidth, "a width of ", width, ": at most ", grace::kNormMaxWidth, " on a GPU");
+  refuse_if<Value>(rows >= INT32_MAX, "at most 2^31 - 2 rows");
   const NormOptions o{gate_rows, post, rms, alpha, eps};
   const bool follow = at::GradMode::is_enabled();
   bool grad = false;
@@ -406,17 +488,18 @@ OptTensor grad_clip(const std::vector<Tensor>& params, int64_t kind, double max_
 }
 
 at::ScalarType scalar_type(const py::object& dtype) {
+  if (!THPDtype_Check(dtype.ptr())) throw py::type_error("dtype must be a torch.dtype");
   return reinterpret_cast<THPDtype*>(dtype.ptr())->scalar_type;
 }
 
 }  // namespace
 
 void grace_bind_lm(py::module& m) {
-  m.def("embedding", [](const Tensor& ids, const Tensor& weight, double scale, int64_t pad, const py::object& dtype) {
-    return embedding(ids, weight, scale, pad, scalar_type(dtype));
+  m.def("embedding", [](const Tensor& ids, const Tensor& weight, double scale, const c10::optional<int64_t>& padding_idx,
+                        const py::object& dtype) {
+    return embedding(ids, weight, scale, padding_idx,
+                     dtype.is_none() ? c10::optional<at::ScalarType>() : scalar_type(dtype));
   });
-  m.attr("embed_max_width") = (int64_t)grace::kEmbedMaxWidth;
-  m.attr("resnorm_max_width") = (int64_t)grace::kNormMaxWidth;
   m.def("residual_norm", &residual_norm);
   m.def("grad_norm_parts", &grad_norm_parts);
   m.def("grad_norm_finish", &grad_norm_finish);

@@ -19,9 +19,6 @@ import torch.nn.functional as F
 
 from . import _native
 
-_DTYPES = (torch.float32, torch.bfloat16, torch.float16)
-
-
 def embedding(ids: torch.Tensor, weight: torch.Tensor, scale: float = 1.0, padding_idx: Optional[int] = None,
               dtype: Optional[torch.dtype] = None) -> torch.Tensor:
     """``round(scale * weight[ids])`` of shape ``[*ids.shape, width]``.
@@ -29,6 +26,8 @@ def embedding(ids: torch.Tensor, weight: torch.Tensor, scale: float = 1.0, paddi
     ``ids``: int64 or int32, any shape and strides.  ``weight``: ``[rows, width]``, float32, bfloat16 or
     float16.  ``dtype``: the output's type (default: the table's).  ``padding_idx`` (negative: from the end)
     names a row that gets no gradient.  Differentiable once, in ``weight``."""
+    if _native.use_native(weight):
+        return _native.lib().embedding(ids, weight, scale, padding_idx, dtype)  # the same refusals, in C++
     if ids.dtype not in (torch.int64, torch.int32):
         raise TypeError(f"embedding: ids must be int64 or int32, got {ids.dtype}")
     if weight.dim() != 2:
@@ -38,22 +37,10 @@ def embedding(ids: torch.Tensor, weight: torch.Tensor, scale: float = 1.0, paddi
     rows = weight.shape[0]
     if rows == 0 and ids.numel() > 0:
         raise ValueError("embedding: the table has no rows")
-    pad = -1
-    if padding_idx is not None:
-        pad = padding_idx + rows if padding_idx < 0 else padding_idx
-        if not 0 <= pad < rows:
-            raise ValueError(f"embedding: padding_idx {padding_idx} outside a table of {rows} rows")
-    dtype = weight.dtype if dtype is None else dtype
-    if _native.use_native(weight):
-        if weight.dtype not in _DTYPES or dtype not in _DTYPES:
-            raise TypeError(f"embedding: float32, bfloat16 or float16 on a GPU, got {weight.dtype} -> {dtype}")
-        if ids.numel() >= 2**31 - 1 or rows >= 2**31 - 1:
-            raise ValueError("embedding: at most 2^31 - 2 tokens and rows")
-        if weight.shape[1] > _native.lib().embed_max_width:
-            raise ValueError(f"embedding: rows of {weight.shape[1]} values: at most {_native.lib().embed_max_width}")
-        return _native.lib().embedding(ids, weight, float(scale), pad, dtype)
+    if padding_idx is not None and not -rows <= padding_idx < rows:
+        raise ValueError(f"embedding: padding_idx {padding_idx} outside a table of {rows} rows")
     wide = weight if weight.dtype == torch.float64 else weight.float()
-    return (F.embedding(ids, wide, None if pad < 0 else pad) * float(scale)).to(dtype)
+    return (F.embedding(ids, wide, padding_idx) * float(scale)).to(weight.dtype if dtype is None else dtype)
 
 
 class ScaledEmbedding(nn.Embedding):

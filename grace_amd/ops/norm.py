@@ -26,8 +26,7 @@ from . import _native
 _DTYPES = (torch.float32, torch.bfloat16, torch.float16)
 
 
-def _gate_rows(gate: torch.Tensor, y: torch.Tensor) -> int:
-    """Consecutive rows of y that share one row of the gate."""
+def _check_gate(gate: torch.Tensor, y: torch.Tensor) -> None:
     lead = y.shape[:-1]
     g = gate.shape[:-1] if gate.dim() == y.dim() else (1,) * len(lead) if gate.dim() == 1 else None
     if g is not None and gate.shape[-1] == y.shape[-1]:
@@ -35,10 +34,7 @@ def _gate_rows(gate: torch.Tensor, y: torch.Tensor) -> int:
         while k < len(lead) and g[k] == lead[k]:
             k += 1
         if all(n == 1 for n in g[k:]):
-            rows = 1
-            for n in lead[k:]:
-                rows *= n
-            return rows
+            return
     raise ValueError(f"residual_norm: a gate of shape {tuple(gate.shape)} for a block of {tuple(y.shape)}: it is "
                      "[width], or the block's shape with 1 in place of trailing dimensions before the last")
 
@@ -65,14 +61,17 @@ def residual_norm(y: torch.Tensor, residual: Optional[torch.Tensor] = None, weig
     before the last (``[batch, 1, width]``: one gate a sample); each float32 or of y's type.  ``alpha``
     scales the residual and has no gradient.  Tensors that are not contiguous are copied first.
     Differentiable once."""
+    if _native.use_native(y):  # the same refusals, in C++
+        out = _native.lib().residual_norm(y, residual, weight, bias, kind, eps, gate, alpha, post, post_weight,
+                                          post_bias, return_sum)
+        return tuple(out) if return_sum else out[0]
     if kind not in ("layer", "rms"):
         raise ValueError(f"residual_norm: kind {kind!r}: 'layer' or 'rms'")
     if y.dim() < 1 or y.shape[-1] < 1:
         raise ValueError(f"residual_norm: a block of shape {tuple(y.shape)}")
     if not post and (post_weight is not None or post_bias is not None):
         raise ValueError("residual_norm: post_weight and post_bias need post=True")
-    native = _native.use_native(y)
-    if y.dtype not in _DTYPES and (native or y.dtype != torch.float64):
+    if y.dtype not in (*_DTYPES, torch.float64):
         raise TypeError(f"residual_norm: a block of {y.dtype}")
     width = y.shape[-1]
     if residual is None:
@@ -94,30 +93,23 @@ def residual_norm(y: torch.Tensor, residual: Optional[torch.Tensor] = None, weig
             raise TypeError(f"residual_norm: {name} of {p.dtype} for a block of {y.dtype}")
         if name != "gate" and p.shape != (width,):
             raise ValueError(f"residual_norm: {name} of shape {tuple(p.shape)} for a width of {width}")
-    gate_rows = y.numel() // width
     if gate is not None:
-        gate_rows = _gate_rows(gate, y)
-    rms, eps, alpha = kind == "rms", float(eps), float(alpha)
+        _check_gate(gate, y)
+    rms = kind == "rms"
+    wide = torch.float64 if y.dtype == torch.float64 else torch.float32
+    w = [None if p is None else p.to(wide) for p in (weight, bias, post_weight, post_bias, gate)]
+    s = y.to(wide)
+    if post:
+        s = _torch_norm(s, w[2], w[3], rms, eps)
+    if gate is not None:
+        s = s * w[4]
+    if residual is not None:
+        s = s + alpha * residual.to(wide)
+    h = _torch_norm(s, w[0], w[1], rms, eps).to(y.dtype)
+    if not return_sum:
+        return h
     plain = residual is None and gate is None and not post
-    if not native:
-        wide = torch.float64 if y.dtype == torch.float64 else torch.float32
-        w = [None if p is None else p.to(wide) for p in (weight, bias, post_weight, post_bias, gate)]
-        s = y.to(wide)
-        if post:
-            s = _torch_norm(s, w[2], w[3], rms, eps)
-        if gate is not None:
-            s = s * w[4]
-        if residual is not None:
-            s = s + alpha * residual.to(wide)
-        h = _torch_norm(s, w[0], w[1], rms, eps).to(y.dtype)
-        return (h, y if plain else s.to(y.dtype if residual is None else residual.dtype)) if return_sum else h
-    if width > _native.lib().resnorm_max_width:
-        raise ValueError(f"residual_norm: a width of {width}: at most {_native.lib().resnorm_max_width} on a GPU")
-    if y.numel() // width >= 2**31 - 1:
-        raise ValueError("residual_norm: at most 2^31 - 2 rows")
-    out = _native.lib().residual_norm(y, residual, gate, gate_rows, weight, bias, post_weight, post_bias, post, rms,
-                                      alpha, eps, return_sum)
-    return tuple(out) if return_sum else out[0]
+    return h, y if plain else s.to(y.dtype if residual is None else residual.dtype)
 
 
 class ResidualNorm(nn.Module):

@@ -13,6 +13,7 @@ from grace_amd.parallel import FusedSGD, clip_grad_norm_, grad_norm
 import lm_oracle as O
 
 F32, BF16, F16, F64 = torch.float32, torch.bfloat16, torch.float16, torch.float64
+DEVICES = ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)]  # a GPU's refusals come from the host too
 
 
 # ---------------------------------------------------------------------------- embedding
@@ -41,24 +42,26 @@ def test_embedding_gradcheck_and_module():
     torch.testing.assert_close(b(ids), a(ids) * 2, rtol=0, atol=0)
 
 
-def test_embedding_refusals():
-    w, ids = torch.randn(4, 3), torch.tensor([1, 2])
+@pytest.mark.parametrize("device", DEVICES)
+def test_embedding_refusals(device):
+    w, ids = torch.randn(4, 3, device=device), torch.tensor([1, 2], device=device)
     for bad in (ids.float(), ids.to(torch.int16), ids.bool()):
         with pytest.raises(TypeError):
             embedding(bad, w)
     with pytest.raises(ValueError):
         embedding(ids, w[0])
     with pytest.raises(ValueError):
-        embedding(ids, torch.empty(0, 3))
+        embedding(ids, torch.empty(0, 3, device=device))
     for pad in (4, -5):
         with pytest.raises(ValueError):
             embedding(ids, w, padding_idx=pad)
-    with pytest.raises(IndexError):
-        embedding(torch.tensor([4]), w)
+    if device == "cpu":
+        with pytest.raises(IndexError):
+            embedding(torch.tensor([4]), w)
     for kw in (dict(max_norm=1.0), dict(sparse=True), dict(scale_grad_by_freq=True)):
         with pytest.raises(ValueError):
             ScaledEmbedding(4, 3, **kw)
-    assert embedding(torch.empty(0, 2, dtype=torch.int64), w).shape == (0, 2, 3)
+    assert embedding(ids.new_empty(0, 2), w).shape == (0, 2, 3)
 
 
 # ---------------------------------------------------------------------------- residual norm
@@ -136,9 +139,13 @@ def test_residual_norm_module_loads_layer_norm():
     assert ResidualNorm(12, bias=False, post=True).post_bias is None
 
 
-def test_residual_norm_refusals():
-    y, x, w = torch.randn(2, 3, 4), torch.randn(2, 3, 4), torch.ones(4)
-    for bad in (torch.ones(3), torch.ones(3, 4), torch.ones(1, 3, 4), torch.ones(2, 3, 1), torch.ones(2, 1, 1, 4)):
+@pytest.mark.parametrize("device", DEVICES)
+def test_residual_norm_refusals(device):
+    def ones(*shape):
+        return torch.ones(shape, device=device)
+
+    y, x, w = ones(2, 3, 4), ones(2, 3, 4), ones(4)
+    for bad in (ones(3), ones(3, 4), ones(1, 3, 4), ones(2, 3, 1), ones(2, 1, 1, 4), ones()):
         with pytest.raises(ValueError):
             residual_norm(y, x, w, gate=bad)
     for kw in (dict(kind="batch"), dict(post_weight=w), dict(post_bias=w)):
@@ -149,11 +156,11 @@ def test_residual_norm_refusals():
     with pytest.raises(ValueError):
         residual_norm(y, x[:1], w)
     with pytest.raises(ValueError):
-        residual_norm(y, x, torch.ones(5))
+        residual_norm(y, x, ones(5))
     with pytest.raises(ValueError):
-        residual_norm(y, x, w, torch.ones(1, 4))
+        residual_norm(y, x, w, ones(1, 4))
     with pytest.raises(ValueError):
-        residual_norm(torch.tensor(1.0))
+        residual_norm(ones())
     with pytest.raises(TypeError):
         residual_norm(y, x.bfloat16(), w)
     with pytest.raises(TypeError):
