@@ -24,13 +24,11 @@ constexpr int64_t kEmbedMaxWidth = 1 << 23;  // slabs of columns are a grid's se
 void embed_forward(const EmbedIds& ids, const void* w, ElType tw, int64_t w_stride, int64_t d, float scale, void* out,
                    ElType to, hipStream_t stream);
 
-// whether embed_backward clears dw itself (16-byte aligned); it expects zeros otherwise
-bool embed_backward_fills(int64_t n);
-
 // bytes of workspace that embed_backward needs
 int64_t embed_backward_ws(int64_t n, int64_t vocab, int64_t d);
 
-// dw[v, :] = round(scale * sum of dy[t, :] over ids[t] == v), every row of dw [vocab, d] written
+// dw[v, :] = round(scale * sum of dy[t, :] over ids[t] == v), every row of dw [vocab, d] (16-byte aligned)
+// written; n > 0
 void embed_backward(const EmbedIds& ids, const void* dy, ElType tdy, int64_t d, float scale, void* dw, ElType tdw,
                     void* ws, hipStream_t stream);
 

@@ -5,14 +5,14 @@
 //
 // The backward sums the rows of equal tokens in token order, so the result does not depend on the launch: no
 // floating-point atomics.  Two ways there, by the number of tokens n:
-//   n <= kFew    a workgroup per token looks through all tokens; the first of its kind sums them all
-//                (one launch after the fill; the reads of n^2 ids stay in L2)
+//   n <= kFew    one launch: a workgroup per token looks through all tokens, and the first of its kind sums them
+//                all; workgroups behind them clear the rows that no token names (the n ids stay in L2)
 //   n >  kFew    the tokens are sorted by row (a stable LSD radix sort of (row, token) pairs, 8 bits a
 //                pass; up to kSmall pairs in the LDS of one workgroup) and cut into chunks; a wave sums
 //                one chunk over a slab of columns in fp32 and writes every run of equal rows inside
 //                it.  Runs that cross a chunk's border (a padding or mask token can fill an eighth of a batch)
 //                leave one partial row per chunk, which a join launch adds in chunk order.
-// dw is filled with zeros by the workgroups that a sort launch leaves idle, so the fill hides the sort.
+// There dw is filled with zeros by the workgroups that a sort launch leaves idle, so the fill hides the sort.
 // Tokens outside [0, vocab) and the padding row sort behind all rows (key = vocab) and are left out; the
 // lookup gives NaN rows for the former, so that a bad token is loud without a host synchronisation.
 #include <algorithm>
@@ -72,15 +72,44 @@ __global__ __launch_bounds__(kBlock) void embed_fwd_kernel(EmbedIds ids, const T
 // ---------------------------------------------------------------- few tokens
 constexpr int kFew = 1024;
 
-// Workgroup (token t, slab of columns).  Each wave looks through a quarter of the tokens and notes those of
-// t's row; if t is the first of them the waves sum their notes and meet in LDS in token order.
+// Clears those of the rows [r0, r1) that no token names: at most kClearRows of them, 2^lanes_log lanes a row.
+constexpr int kClearRows = 1024;
+template <typename TG>
+__device__ __forceinline__ void clear_rows(const EmbedIds& ids, int64_t r0, int64_t r1, int64_t d, int lanes_log,
+                                           TG* __restrict__ dw) {
+  constexpr int V = 16 / sizeof(TG);
+  __shared__ uint32_t named[kClearRows / 32];
+  for (int i = threadIdx.x; i < kClearRows / 32; i += kBlock) named[i] = 0;
+  __syncthreads();
+  for (int i = threadIdx.x; i < (int)ids.n; i += kBlock) {
+    const int64_t id = id_at(ids, i);
+    if (id >= r0 && id < r1 && id != ids.pad) atomicOr(&named[(id - r0) / 32], 1u << ((id - r0) & 31));
+  }
+  __syncthreads();
+  const int lane = threadIdx.x & ((1 << lanes_log) - 1);
+  const float zero[V] = {};
+  for (int64_t r = r0 + (threadIdx.x >> lanes_log); r < r1; r += kBlock >> lanes_log) {
+    if (named[(r - r0) / 32] >> ((r - r0) & 31) & 1) continue;
+    for (int64_t c = (int64_t)lane * V; c < d; c += (int64_t)V << lanes_log)
+      store_vec(dw + r * d + c, zero, (int)min(d - c, (int64_t)V));
+  }
+}
+
+// Workgroup (token t, slab of columns), and behind those the ones that clear.  Each wave looks through a quarter of
+// the tokens and notes those of t's row; if t is the first of them the waves sum their notes and meet in LDS
+// in token order.
 template <typename TD, typename TG>
 __global__ __launch_bounds__(kBlock) void embed_few_kernel(EmbedIds ids, const TD* __restrict__ dy, int64_t d,
-                                                           float scale, TG* __restrict__ dw) {
+                                                           float scale, TG* __restrict__ dw, int slabs, int rows_each,
+                                                           int lanes_log) {
   constexpr int V = vec_of<TD, float>(), kSlab = kWave * V, U = 8;
+  const int n = (int)ids.n, w = wave_id();
+  const int64_t clear = (int64_t)blockIdx.x - (int64_t)n * slabs;
+  if (clear >= 0)
+    return clear_rows(ids, clear * rows_each, min((clear + 1) * rows_each, ids.vocab), d, lanes_log, dw);
   __shared__ uint16_t note[kWaves][kFew / kWaves];
   __shared__ float part[kWaves][kSlab];
-  const int t = blockIdx.x, n = (int)ids.n, w = wave_id();
+  const int t = blockIdx.x % n;
   const int64_t id = id_at(ids, t);
   if (id < 0 || id >= ids.vocab || id == ids.pad) return;
   const int quarter = (n + kWaves - 1) / kWaves, begin = w * quarter, end = min(begin + quarter, n);
@@ -94,7 +123,7 @@ __global__ __launch_bounds__(kBlock) void embed_few_kernel(EmbedIds ids, const T
     earlier |= same && i < t;
   }
   if (__syncthreads_or(earlier)) return;
-  const int64_t col = (int64_t)blockIdx.y * kSlab + lane_id() * V;
+  const int64_t col = (int64_t)(blockIdx.x / n) * kSlab + lane_id() * V;
   const int left = (int)max(min(d - col, (int64_t)V), (int64_t)0);
   float acc[V] = {};
   for (int j0 = 0; j0 < found; j0 += U) {
@@ -534,8 +563,6 @@ void embed_forward(const EmbedIds& ids, const void* w, ElType tw, int64_t w_stri
   });
 }
 
-bool embed_backward_fills(int64_t n) { return n > kFew; }
-
 int64_t embed_backward_ws(int64_t n, int64_t vocab, int64_t d) {
   if (n <= kFew) return 0;
   const Plan p = plan_of(n);
@@ -552,8 +579,13 @@ void embed_backward(const EmbedIds& ids, const void* dy, ElType tdy, int64_t d, 
       using TG = std::remove_pointer_t<decltype(tag_g)>;
       by_type(tdy, [&](auto* tag_d) {
         using TD = std::remove_pointer_t<decltype(tag_d)>;
-        const unsigned slabs = (unsigned)cdiv(d, kWave * vec_of<TD, float>());
-        embed_few_kernel<TD, TG><<<dim3((unsigned)n, slabs), kBlock, 0, stream>>>(ids, (const TD*)dy, d, scale, (TG*)dw);
+        const int64_t slabs = cdiv(d, kWave * vec_of<TD, float>());
+        // about 64 KB to clear for a workgroup: the ids that it reads for it are at most an eighth of that
+        const int64_t each = std::max<int64_t>(1, std::min<int64_t>(kClearRows, 65536 / (d * (int64_t)sizeof(TG))));
+        int log = 0;
+        while (log < 8 && ((int64_t)(16 / sizeof(TG)) << log) < d) ++log;
+        embed_few_kernel<TD, TG><<<(unsigned)(n * slabs + cdiv(ids.vocab, each)), kBlock, 0, stream>>>(
+            ids, (const TD*)dy, d, scale, (TG*)dw, (int)slabs, (int)each, log);
       });
     });
     return;

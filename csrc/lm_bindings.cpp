@@ -68,10 +68,12 @@ Tensor embed_bwd(const Tensor& ids, const Tensor& dy, int64_t vocab, int64_t pad
   const grace::EmbedIds e = embed_ids(ids, vocab, d, pad);
   DevGuard guard(dy.device());
   const auto tdw = el_type(dtype, "embedding: the table"), tdy = el_type(dy.scalar_type(), "embedding: the gradient");
-  Tensor dw = grace::embed_backward_fills(e.n) ? at::empty({vocab, d}, dy.options().dtype(dtype))
-                                               : at::zeros({vocab, d}, dy.options().dtype(dtype));
-  Tensor ws = at::empty({grace::embed_backward_ws(e.n, vocab, d)}, dy.options().dtype(at::kByte));
-  grace::embed_backward(e, dy.data_ptr(), tdy, d, (float)scale, dw.data_ptr(), tdw, ws.data_ptr(), cur_stream());
+  if (e.n == 0 || vocab == 0 || d == 0) return at::zeros({vocab, d}, dy.options().dtype(dtype));
+  Tensor dw = at::empty({vocab, d}, dy.options().dtype(dtype));
+  const int64_t bytes = grace::embed_backward_ws(e.n, vocab, d);
+  const Tensor ws = bytes > 0 ? at::empty({bytes}, dy.options().dtype(at::kByte)) : Tensor();
+  grace::embed_backward(e, dy.data_ptr(), tdy, d, (float)scale, dw.data_ptr(), tdw,
+                        bytes > 0 ? ws.data_ptr() : nullptr, cur_stream());
   C10_HIP_KERNEL_LAUNCH_CHECK();
   return dw;
 }
