@@ -11,14 +11,19 @@
 //        dpw = sum du . y^,  dpb = sum du
 //
 // A row lives in registers (E values per thread), so every input is read once and the variance is
-// taken about the mean in a second sweep over registers.  64, 256, 512 or 1024 threads share a row,
-// by its width; a workgroup walks over rows with the weights in registers, and rows that need a
-// workgroup's barriers are loaded one ahead.  Statistics and sums are fp32; s is rounded to its own
+// taken about the mean in a second sweep over registers.  16, 64, 256, 512 or 1024 threads share a row,
+// by its width; a workgroup walks over rows with the weights at hand, and rows that need a workgroup's
+// barriers are loaded one ahead.  Statistics and sums are fp32; s is rounded to its own
 // type only where it is stored, and h is made from the unrounded sum.  The backward reads the stored
 // sum if that is fp32; a 16-bit sum is made again from x and y, because its rounding would show in
 // the fp32 sums dw (2^-9 of every term against 2^-24).
 // Column sums (dw, db, dgate, dpw, dpb): every workgroup adds up its rows in registers and leaves one
 // partial row; a second launch adds the partial rows in a fixed order.
+//
+// Bound by memory: a copy runs at 5.2 TB/s.  64 million values in whole vectors, forward and backward: bf16 widths of
+// 256 to 8192 at 5.0-5.6 and 4.2-4.4 TB/s, fp32 at 4.6-5.5 and 4.6-4.9.  What does not reach that: a norm before and
+// behind with a gate keeps five sums and four weights a value, which 1024 threads of 128 registers do not hold
+// (backward, 12000 columns: 0.8 TB/s in bf16, 2.0 in fp32; up to 8192 columns 3.3-4.8).
 #pragma once
 
 #include <algorithm>
@@ -36,8 +41,11 @@ constexpr int kCUs = 256;
 template <int TPR>
 constexpr int block_of() { return TPR < 256 ? 256 : TPR; }
 
-// values per load: 16 bytes of the narrower type
-template <typename TX, typename TY>
+// Values per load: 16 bytes of the narrower type where the rows are whole vectors.  A row that ends inside one is
+// taken by single values, so that a wave's accesses are aligned and next to each other: wide ones of 16-bit values at
+// odd addresses run at half the rate, and the branches of a partial vector cost registers and waits (bf16, forward
+// and backward: 1100 columns 3.6 and 2.8 TB/s, as vectors 2.3 and 2.4; 651 columns 4.1 and 3.7 for 3.5 and 3.8).
+template <typename TY>
 constexpr int vec_of() { return sizeof(TY) == 2 ? 8 : 4; }
 
 struct FwdArgs {
@@ -91,6 +99,17 @@ __device__ __forceinline__ float dpp_sum(float v) {
   return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63));
 }
 
+// Sum over 16 lanes, in each of them: rotations within the row of lanes.
+__device__ __forceinline__ float dpp_sum16(float v) {
+#define GRACE_ROR(n) v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x120 + n, 0xf, 0xf, true))
+  GRACE_ROR(8);
+  GRACE_ROR(4);
+  GRACE_ROR(2);
+  GRACE_ROR(1);
+#undef GRACE_ROR
+  return v;
+}
+
 // Sums over the TPR threads of a row.  More than one wave: one barrier a sum, on two buffers in turn
 // (a wave can be at most one barrier ahead of another).
 template <int TPR>
@@ -99,8 +118,8 @@ struct RowSum {
   float* scratch;  // [2][2 W]
   int turn = 0;
   __device__ __forceinline__ void operator()(float& a, float& b) {
-    a = dpp_sum(a);
-    b = dpp_sum(b);
+    a = TPR == 16 ? dpp_sum16(a) : dpp_sum(a);
+    b = TPR == 16 ? dpp_sum16(b) : dpp_sum(b);
     if constexpr (W > 1) {
       float* q = scratch + turn * 2 * W;
       turn ^= 1;
@@ -129,48 +148,67 @@ struct Raw {
   Bits<T, V> v[J];
 };
 
+// The width is a multiple of V.
 template <int TPR, int V, int J>
 struct Row {
   int t, d;
-  int left[J];  // values of vector j inside the width (at most 0: none)
-  __device__ __forceinline__ Row(int t, int d) : t(t), d(d) {
-#pragma unroll
-    for (int j = 0; j < J; ++j) left[j] = min(d - (j * TPR + t) * V, V);
-  }
+  __device__ __forceinline__ Row(int t, int d) : t(t), d(d) {}
   __device__ __forceinline__ int col(int j) const { return (j * TPR + t) * V; }
+  __device__ __forceinline__ bool in(int j) const { return col(j) < d; }  // vector j is inside the width
 
   // as stored; zero outside the width, or everywhere without a pointer
   template <typename T>
   __device__ __forceinline__ void load(const void* p, int64_t at, Raw<T, V, J>& r) const {
 #pragma unroll
-    for (int j = 0; j < J; ++j) {
+    for (int j = 0; j < J; ++j)
 #pragma unroll
       for (int i = 0; i < Bits<T, V>::W; ++i) r.v[j].w[i] = 0;
-      if (p != nullptr && left[j] > 0) load_bits(static_cast<const T*>(p) + at + col(j), r.v[j], left[j]);
-    }
+    // asked once of 8 or 16 single values, but of every vector: two or four of them run better so
+    const bool there = p != nullptr;
+    if (V == 1 && !there) return;
+#pragma unroll
+    for (int j = 0; j < J; ++j)
+      if ((V == 1 || there) && in(j)) load_bits(static_cast<const T*>(p) + at + col(j), r.v[j]);
   }
-  template <typename TY>
-  __device__ __forceinline__ void param(const NormParam& p, int64_t at, float none, float (&o)[J][V]) const {
+  // Before the first use of r: single 16-bit values are widened behind this, not where each is loaded, which would
+  // make every load wait for the one before it.
+  template <typename T>
+  __device__ __forceinline__ void arrive(Raw<T, V, J>& r) const {
+    if constexpr (V == 1 && sizeof(T) == 2) {
 #pragma unroll
-    for (int j = 0; j < J; ++j) {
-#pragma unroll
-      for (int i = 0; i < V; ++i) o[j][i] = none;
-      if (p.p == nullptr || left[j] <= 0) continue;
-      if (p.f32) load_vec(static_cast<const float*>(p.p) + at + col(j), o[j], left[j]);
-      else load_vec(static_cast<const TY*>(p.p) + at + col(j), o[j], left[j]);
+      for (int j = 0; j < J; ++j) asm volatile("" : "+v"(r.v[j].w[0]));
     }
   }
   template <typename T>
+  __device__ __forceinline__ void widened(const void* p, int64_t at, float (&o)[J][V]) const {
+    Raw<T, V, J> r;
+    load<T>(p, at, r);
+    arrive(r);
+#pragma unroll
+    for (int j = 0; j < J; ++j)
+#pragma unroll
+      for (int i = 0; i < V; ++i) o[j][i] = bits_at(r.v[j], i);
+  }
+  // widened; zero outside the width
+  template <typename TY>
+  __device__ __forceinline__ void param(const NormParam& p, int64_t at, float (&o)[J][V]) const {
+    if (p.f32) widened<float>(p.p, at, o);
+    else widened<TY>(p.p, at, o);
+  }
+  template <typename T>
   __device__ __forceinline__ void store(void* p, int64_t at, const float (&v)[J][V], bool once) const {
-    if (once) {
+    // single values leave lines in parts, for the cache to join (fp32, 130 columns: 280 us past it, 235 us through it)
+    if constexpr (V > 1) {
+      if (once) {
 #pragma unroll
-      for (int j = 0; j < J; ++j)
-        if (left[j] > 0) store_vec<true>(static_cast<T*>(p) + at + col(j), v[j], left[j]);
-    } else {
-#pragma unroll
-      for (int j = 0; j < J; ++j)
-        if (left[j] > 0) store_vec(static_cast<T*>(p) + at + col(j), v[j], left[j]);
+        for (int j = 0; j < J; ++j)
+          if (in(j)) store_vec<true>(static_cast<T*>(p) + at + col(j), v[j]);
+        return;
+      }
     }
+#pragma unroll
+    for (int j = 0; j < J; ++j)
+      if (in(j)) store_vec<false>(static_cast<T*>(p) + at + col(j), v[j]);
   }
   // mean and 1 / deviation of v, which is zero outside the width
   __device__ __forceinline__ void stats(const float (&v)[J][V], bool rms, float eps, RowSum<TPR>& sum, float& mean,
@@ -188,13 +226,9 @@ struct Row {
     a = 0.f;
 #pragma unroll
     for (int j = 0; j < J; ++j) {
-      if (left[j] >= V) {
+      if (in(j)) {
 #pragma unroll
         for (int i = 0; i < V; ++i) a = fmaf(v[j][i] - mean, v[j][i] - mean, a);
-      } else {
-#pragma unroll
-        for (int i = 0; i < V; ++i)
-          if (i < left[j]) a = fmaf(v[j][i] - mean, v[j][i] - mean, a);
       }
     }
     sum(a);
@@ -204,61 +238,86 @@ struct Row {
   __device__ __forceinline__ void trim(float (&v)[J][V]) const {
 #pragma unroll
     for (int j = 0; j < J; ++j)
-      if (left[j] < V) {
+      if (!in(j)) {
 #pragma unroll
-        for (int i = 0; i < V; ++i) v[j][i] = i < left[j] ? v[j][i] : 0.f;
+        for (int i = 0; i < V; ++i) v[j][i] = 0.f;
       }
   }
 };
 
-// The weights (and in the backward the gate) of a workgroup's rows, each thread's own values.  Rows that
-// take a workgroup keep them in LDS, where they cost no registers: the registers decide how many such
-// rows a CU has in flight.  Only the thread that wrote a value reads it, so there are no barriers.
-// 16384 columns would take 64 KB an array, so rows of 16 values a thread keep them in registers.
-template <int K, int TPR, int V, int J, bool LDS>
+// Where the weights and the gate of a workgroup's rows are, each thread's own values of them.
+//   registers  rows of a wave or less
+//   LDS        rows of a workgroup, where they cost no registers: the registers decide how many such rows a CU has
+//              in flight.  Only the thread that wrote a value reads it, so there are no barriers.  An array
+//              takes 16 KB for rows of 512 threads and 8 values, 32 KB for 1024 threads.
+//   memory     rows of 16 values for each of 1024 threads, whose registers and LDS hold no more: from the caches
+enum Home { kInRegisters, kInLds, kInMemory };
+
+template <int K, int TPR, int V, int J, Home HOME>
 struct Params {
-  static constexpr bool kLds = LDS;
-  static constexpr int kFloats = kLds ? TPR * V * J : 0;  // of LDS, for each array
-  float r[kLds ? 1 : K][J][V];
-  float4* lds;
-  __device__ __forceinline__ explicit Params(float* p) : lds(reinterpret_cast<float4*>(p) + threadIdx.x) {}
-  // k: the array (a constant), at: its place in LDS
-  __device__ __forceinline__ void set(int k, int at, const float (&v)[J][V]) {
+  static constexpr int kFloats = HOME == kInLds ? TPR * V * J : 0;  // of LDS, for each array
+  static constexpr int kAccess = V < 4 ? V : 4;                     // values of an LDS access
+  struct alignas(4 * kAccess) Part {
+    float v[kAccess];
+  };
+  float r[HOME == kInRegisters ? K : 1][J][V];
+  Part* lds;
+  __device__ __forceinline__ explicit Params(float* p) : lds(reinterpret_cast<Part*>(p) + threadIdx.x) {}
+  __device__ __forceinline__ Part& part(int place, int j, int i) const {
+    return lds[((place * J + j) * (V / kAccess) + i / kAccess) * TPR];
+  }
+  // k: the array (a constant), place: its place in LDS, from + at: where it is in memory
+  template <typename TY>
+  __device__ __forceinline__ void set(int k, int place, const Row<TPR, V, J>& row, const NormParam& from, int64_t at) {
+    if constexpr (HOME == kInMemory) return;
+    float v[J][V];
+    row.template param<TY>(from, at, v);
 #pragma unroll
     for (int j = 0; j < J; ++j)
 #pragma unroll
-      for (int i = 0; i < V; i += 4) {
-        if constexpr (kLds) {
-          lds[((at * J + j) * (V / 4) + i / 4) * TPR] = make_float4(v[j][i], v[j][i + 1], v[j][i + 2], v[j][i + 3]);
+      for (int i = 0; i < V; i += kAccess) {
+        Part q;
+#pragma unroll
+        for (int m = 0; m < kAccess; ++m) q.v[m] = v[j][i + m];
+        if constexpr (HOME == kInLds) {
+          part(place, j, i) = q;
         } else {
 #pragma unroll
-          for (int q = 0; q < 4; ++q) r[k][j][i + q] = v[j][i + q];
+          for (int m = 0; m < kAccess; ++m) r[k][j][i + m] = q.v[m];
         }
       }
   }
-  __device__ __forceinline__ void get(int k, int at, float (&v)[J][V]) const {
+  template <typename TY>
+  __device__ __forceinline__ void get(int k, int place, const Row<TPR, V, J>& row, const NormParam& from, int64_t at,
+                                      float (&v)[J][V]) const {
+    if constexpr (HOME == kInMemory) {
+      int64_t none = 0;  // which the compiler can't see: it would keep single values in registers, 16 for each array
+      if constexpr (V == 1) asm volatile("" : "+s"(none));
+      row.template param<TY>(from, at + none, v);
+    } else {
 #pragma unroll
-    for (int j = 0; j < J; ++j)
+      for (int j = 0; j < J; ++j)
 #pragma unroll
-      for (int i = 0; i < V; i += 4) {
-        if constexpr (kLds) {
-          const float4 q = lds[((at * J + j) * (V / 4) + i / 4) * TPR];
-          v[j][i] = q.x;
-          v[j][i + 1] = q.y;
-          v[j][i + 2] = q.z;
-          v[j][i + 3] = q.w;
-        } else {
+        for (int i = 0; i < V; i += kAccess) {
+          if constexpr (HOME == kInLds) {
+            const Part q = part(place, j, i);
 #pragma unroll
-          for (int q = 0; q < 4; ++q) v[j][i + q] = r[k][j][i + q];
+            for (int m = 0; m < kAccess; ++m) v[j][i + m] = q.v[m];
+          } else {
+#pragma unroll
+            for (int m = 0; m < kAccess; ++m) v[j][i + m] = r[k][j][i + m];
+          }
         }
-      }
+    }
   }
 };
 
-// the workgroup's slot of rows, known to be the same in a wave
+// the workgroup's slot of rows; known to be the same in a wave where it is
 template <int TPR>
 __device__ __forceinline__ int row_slot() {
-  return block_of<TPR>() == TPR ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x / TPR);
+  if constexpr (block_of<TPR>() == TPR) return 0;
+  else if constexpr (TPR < kWave) return threadIdx.x / TPR;
+  else return __builtin_amdgcn_readfirstlane(threadIdx.x / TPR);
 }
 
 enum { kW, kB, kPw, kPb, kG, kParams };
@@ -274,19 +333,23 @@ struct ParamPlaces {
   }
 };
 
+// Forward: rows of a wave or less take the weights from the caches, so that few registers let many rows run at once
+// (16 values a thread and the weights in registers: 160 registers, two rounds for 4096 rows).  At most five
+// arrays in LDS, 80 KB; 1024 threads would take 160 KB and have registers enough.
+template <int TPR>
+constexpr Home forward_home() { return TPR <= kWave ? kInMemory : TPR < 1024 ? kInLds : kInRegisters; }
+// Backward: at most four arrays in LDS, 128 KB.
 template <int E, int TPR>
-constexpr bool lds_forward() { return TPR > kWave && TPR < 1024; }  // at most five arrays: 80 KB
-template <int E, int TPR>
-constexpr bool lds_backward() { return TPR > kWave && E == 8; }  // at most four: 128 KB
+constexpr Home backward_home() { return TPR <= kWave ? kInRegisters : E == 8 ? kInLds : kInMemory; }
 
 #define GRACE_EACH(body)          \
   _Pragma("unroll") for (int j = 0; j < J; ++j) \
   _Pragma("unroll") for (int i = 0; i < V; ++i) { body; }
 
 // ---------------------------------------------------------------- forward
-template <typename TX, typename TY, int E, int TPR>
+template <typename TX, typename TY, int E, int TPR, int V>
 __global__ __launch_bounds__(block_of<TPR>()) void resnorm_fwd_kernel(FwdArgs g) {
-  constexpr int V = vec_of<TX, TY>(), J = E / V, kSlots = block_of<TPR>() / TPR;
+  constexpr int J = E / V, kSlots = block_of<TPR>() / TPR;
   __shared__ float scratch[TPR > kWave ? 4 * TPR / kWave : 1];
   RowSum<TPR> sum{scratch};
   const NormShape& n = g.n;
@@ -294,8 +357,6 @@ __global__ __launch_bounds__(block_of<TPR>()) void resnorm_fwd_kernel(FwdArgs g)
   const uint32_t rows = (uint32_t)n.rows, step = gridDim.x * kSlots, gate_rows = (uint32_t)n.gate_rows;
   uint32_t r = blockIdx.x * kSlots + row_slot<TPR>();
   if (r >= rows) return;
-  // Rows of one wave: many are in flight anyway, and few registers (78 for 160) let all 4096 rows of a
-  // small batch run at once; their weights come from the caches.
   constexpr bool AHEAD = TPR > kWave;
   Raw<TY, V, J> ry;
   Raw<TX, V, J> rx;
@@ -305,35 +366,30 @@ __global__ __launch_bounds__(block_of<TPR>()) void resnorm_fwd_kernel(FwdArgs g)
   };
   fetch(r);
   extern __shared__ __align__(16) float dyn[];
-  Params<kParams, TPR, V, J, lds_forward<E, TPR>()> params(dyn);
-  const ParamPlaces at_lds(g.weight.p, g.bias.p, g.gate.p, n.post ? g.post_weight.p : nullptr,
+  Params<kParams, TPR, V, J, forward_home<TPR>()> params(dyn);
+  const ParamPlaces places(g.weight.p, g.bias.p, g.gate.p, n.post ? g.post_weight.p : nullptr,
                            n.post ? g.post_bias.p : nullptr);
-  {
-    float v[J][V];
-    auto put = [&](int k, const NormParam& p, float none) {
-      if (!AHEAD || at_lds.at[k] < 0) return;
-      row.template param<TY>(p, 0, none, v);
-      params.set(k, at_lds.at[k], v);
-    };
-    put(kW, g.weight, 1.f);
-    put(kB, g.bias, 0.f);
-    put(kPw, g.post_weight, 1.f);
-    put(kPb, g.post_bias, 0.f);
-  }
+  auto put = [&](int k, const NormParam& from) {
+    if (places.at[k] >= 0) params.template set<TY>(k, places.at[k], row, from, 0);
+  };
+  put(kW, g.weight);
+  put(kB, g.bias);
+  put(kPw, g.post_weight);
+  put(kPb, g.post_bias);
   auto take = [&](int k, const NormParam& from, float(&v)[J][V]) {
-    if constexpr (AHEAD) params.get(k, at_lds.at[k], v);
-    else row.template param<TY>(from, 0, 0.f, v);
+    params.template get<TY>(k, places.at[k], row, from, 0, v);
   };
   uint32_t gate_now = ~0u;
   for (;;) {
     const int64_t at = (int64_t)r * n.d;
-    float u[J][V], x[J][V], p[J][V], gate[J][V], mean, rstd;
+    float u[J][V], x[J][V], p[J][V], mean, rstd;
     // a gate that stays is not loaded again: a load here would make the row wait for the last one's stores
-    if (g.gate.p != nullptr && (!AHEAD || r / gate_rows != gate_now)) {
+    if (g.gate.p != nullptr && r / gate_rows != gate_now) {
       gate_now = r / gate_rows;
-      row.template param<TY>(g.gate, (int64_t)gate_now * n.d, 1.f, gate);
-      if (AHEAD) params.set(kG, at_lds.at[kG], gate);
+      params.template set<TY>(kG, places.at[kG], row, g.gate, (int64_t)gate_now * n.d);
     }
+    row.arrive(ry);
+    row.arrive(rx);
     GRACE_EACH(u[j][i] = bits_at(ry.v[j], i); x[j][i] = bits_at(rx.v[j], i))
     const bool more = rows - r > step;
     if (AHEAD && more) fetch(r + step);
@@ -354,8 +410,8 @@ __global__ __launch_bounds__(block_of<TPR>()) void resnorm_fwd_kernel(FwdArgs g)
       }
     }
     if (g.gate.p != nullptr) {
-      if (AHEAD) params.get(kG, at_lds.at[kG], gate);
-      GRACE_EACH(u[j][i] *= gate[j][i])
+      params.template get<TY>(kG, places.at[kG], row, g.gate, (int64_t)gate_now * n.d, p);
+      GRACE_EACH(u[j][i] *= p[j][i])
     }
     if (g.x != nullptr) GRACE_EACH(u[j][i] = fmaf(n.alpha, x[j][i], u[j][i]))
     row.trim(u);
@@ -383,12 +439,12 @@ __global__ __launch_bounds__(block_of<TPR>()) void resnorm_fwd_kernel(FwdArgs g)
 
 // ---------------------------------------------------------------- backward
 template <typename TY, int V>
-__device__ __forceinline__ void store_param(void* p, bool f32, int64_t at, const float (&v)[V], int n) {
-  if (f32) store_vec(static_cast<float*>(p) + at, v, n);
-  else store_vec(static_cast<TY*>(p) + at, v, n);
+__device__ __forceinline__ void store_param(void* p, bool f32, int64_t at, const float (&v)[V]) {
+  if (f32) store_vec(static_cast<float*>(p) + at, v);
+  else store_vec(static_cast<TY*>(p) + at, v);
 }
 
-// Sums acc over the workgroup's row slots and hands each vector to out(column, values, count); acc
+// Sums acc over the workgroup's row slots and hands each vector to out(column, values); acc
 // is left as it is.  red: [slots][TPR * E] floats for more than one slot.
 template <int TPR, int V, int J, typename F>
 __device__ __forceinline__ void over_slots(const float (&acc)[J][V], const Row<TPR, V, J>& row, float* red, F&& out) {
@@ -405,20 +461,23 @@ __device__ __forceinline__ void over_slots(const float (&acc)[J][V], const Row<T
 #pragma unroll
         for (int k = 1; k < kSlots; ++k) v[i] += red[k * kRow + c + i];
       }
-      out(c, v, min(row.d - c, V));
+      out(c, v);
     }
   } else {
 #pragma unroll
     for (int j = 0; j < J; ++j)
-      if (row.left[j] > 0) out(row.col(j), acc[j], row.left[j]);
+      if (row.in(j)) out(row.col(j), acc[j]);
   }
 }
 
 // BIAS: one of the two biases is there
-template <typename TX, typename TY, int E, int TPR, bool POST, bool GATED, bool BIAS>
+template <typename TX, typename TY, int E, int TPR, int V, bool POST, bool GATED, bool BIAS>
 __global__ __launch_bounds__(block_of<TPR>(), TPR == 512 ? 4 : 1) void resnorm_bwd_kernel(BwdArgs g) {
-  constexpr int V = vec_of<TX, TY>(), J = E / V, kSlots = block_of<TPR>() / TPR;
-  constexpr bool AHEAD = TPR > kWave;  // the next row's loads are issued before this row's sums
+  constexpr int J = E / V, kSlots = block_of<TPR>() / TPR;
+  // The next row's loads are issued before this row's sums, where registers hold them: 1024 threads have 128 each,
+  // and a single 16-bit value takes as much of them as two in a vector.
+  constexpr bool AHEAD =
+      TPR > kWave && E == 8 && !(TPR == 1024 && sizeof(TY) == 4 && (POST || GATED)) && !(V == 1 && sizeof(TY) == 2);
   __shared__ float scratch[TPR > kWave ? 4 * TPR / kWave : 1];
   __shared__ float red[kSlots > 1 ? kSlots * TPR * E : 1];
   RowSum<TPR> sum{scratch};
@@ -427,28 +486,15 @@ __global__ __launch_bounds__(block_of<TPR>(), TPR == 512 ? 4 : 1) void resnorm_b
   float dw[J][V], db[J][V], dg[J][V], dpw[J][V], dpb[J][V];
   GRACE_EACH(dw[j][i] = db[j][i] = dg[j][i] = dpw[j][i] = dpb[j][i] = 0.f)
   extern __shared__ __align__(16) float dyn[];
-  Params<2 + 2 * POST, TPR, V, J, lds_backward<E, TPR>()> params(dyn);
+  Params<2 + 2 * POST, TPR, V, J, backward_home<E, TPR>()> params(dyn);
   constexpr int W = 0, G = 1, PW = 2, PB = 3;  // the places in registers
-  const ParamPlaces at_lds(g.weight.p, nullptr, g.gate.p, POST ? g.post_weight.p : nullptr,
+  const ParamPlaces places(g.weight.p, nullptr, g.gate.p, POST ? g.post_weight.p : nullptr,
                            POST && BIAS ? g.post_bias.p : nullptr);
-  {
-    float v[J][V];
-    if (g.weight.p != nullptr) {
-      row.template param<TY>(g.weight, 0, 1.f, v);
-      params.set(W, at_lds.at[kW], v);
-    }
-    if constexpr (POST) {
-      if (g.post_weight.p != nullptr) {
-        row.template param<TY>(g.post_weight, 0, 1.f, v);
-        params.set(PW, at_lds.at[kPw], v);
-      }
-      if constexpr (BIAS) {
-        if (g.post_bias.p != nullptr) {
-          row.template param<TY>(g.post_bias, 0, 0.f, v);
-          params.set(PB, at_lds.at[kPb], v);
-        }
-      }
-    }
+  if (g.weight.p != nullptr) params.template set<TY>(W, places.at[kW], row, g.weight, 0);
+  if constexpr (POST) {
+    if (g.post_weight.p != nullptr) params.template set<TY>(PW, places.at[kPw], row, g.post_weight, 0);
+    if constexpr (BIAS)
+      if (g.post_bias.p != nullptr) params.template set<TY>(PB, places.at[kPb], row, g.post_bias, 0);
   }
   const bool again = sizeof(TX) == 2 && g.s == nullptr;
   const void* sx = again ? g.x : g.s;
@@ -481,9 +527,7 @@ __global__ __launch_bounds__(block_of<TPR>(), TPR == 512 ? 4 : 1) void resnorm_b
       if constexpr (GATED) {
         if (r / gate_rows != gate_now) {
           gate_now = r / gate_rows;
-          float v[J][V];
-          row.template param<TY>(g.gate, (int64_t)gate_now * n.d, 1.f, v);
-          params.set(G, at_lds.at[kG], v);
+          params.template set<TY>(G, places.at[kG], row, g.gate, (int64_t)gate_now * n.d);
         }
       }
       float S[J][V], hat[J][V], phat[J][V], ds[J][V], p[J][V];
@@ -492,18 +536,22 @@ __global__ __launch_bounds__(block_of<TPR>(), TPR == 512 ? 4 : 1) void resnorm_b
         GRACE_EACH(u[j][i] = phat[j][i])
         if constexpr (POST) {
           if (g.post_weight.p != nullptr) {
-            params.get(PW, at_lds.at[kPw], p);
+            params.template get<TY>(PW, places.at[kPw], row, g.post_weight, 0, p);
             GRACE_EACH(u[j][i] *= p[j][i])
           }
           if constexpr (BIAS) {
             if (g.post_bias.p != nullptr) {
-              params.get(PB, at_lds.at[kPb], p);
+              params.template get<TY>(PB, places.at[kPb], row, g.post_bias, 0, p);
               GRACE_EACH(u[j][i] += p[j][i])
             }
           }
         }
       };
       float c1 = 0.f, c2 = 0.f;
+      row.arrive(ry);
+      row.arrive(rs);
+      row.arrive(rdh);
+      row.arrive(rds);
       GRACE_EACH(phat[j][i] = bits_at(ry.v[j], i); hat[j][i] = bits_at(rs.v[j], i); S[j][i] = bits_at(rdh.v[j], i);
                  ds[j][i] = bits_at(rds.v[j], i))
       if (AHEAD && r + kSlots < r_end) fetch(r + kSlots);
@@ -512,7 +560,7 @@ __global__ __launch_bounds__(block_of<TPR>(), TPR == 512 ? 4 : 1) void resnorm_b
         float u[J][V];
         made_u(u);
         if constexpr (GATED) {
-          params.get(G, at_lds.at[kG], p);
+          params.template get<TY>(G, places.at[kG], row, g.gate, (int64_t)gate_now * n.d, p);
           GRACE_EACH(u[j][i] *= p[j][i])
         }
         GRACE_EACH(hat[j][i] = fmaf(n.alpha, hat[j][i], u[j][i]))
@@ -520,7 +568,7 @@ __global__ __launch_bounds__(block_of<TPR>(), TPR == 512 ? 4 : 1) void resnorm_b
       GRACE_EACH(hat[j][i] = (hat[j][i] - mean) * rstd; dw[j][i] = fmaf(S[j][i], hat[j][i], dw[j][i]))
       if constexpr (BIAS) GRACE_EACH(db[j][i] += S[j][i])
       if (g.weight.p != nullptr) {
-        params.get(W, at_lds.at[kW], p);
+        params.template get<TY>(W, places.at[kW], row, g.weight, 0, p);
         GRACE_EACH(S[j][i] *= p[j][i])
       }
       GRACE_EACH(c1 += S[j][i]; c2 = fmaf(S[j][i], hat[j][i], c2))
@@ -538,13 +586,13 @@ __global__ __launch_bounds__(block_of<TPR>(), TPR == 512 ? 4 : 1) void resnorm_b
       if constexpr (GATED) {
         float u[J][V];
         made_u(u);
-        params.get(G, at_lds.at[kG], p);
+        params.template get<TY>(G, places.at[kG], row, g.gate, (int64_t)gate_now * n.d, p);
         GRACE_EACH(u[j][i] *= S[j][i]; dg[j][i] = g.dgate_mode == kGateRows ? u[j][i] : dg[j][i] + u[j][i];
                    S[j][i] *= p[j][i])
         if (g.dgate_mode == kGateRows) {
 #pragma unroll
           for (int j = 0; j < J; ++j)
-            if (row.left[j] > 0) store_param<TY>(g.dgate, g.dgate_f32, at + row.col(j), dg[j], row.left[j]);
+            if (row.in(j)) store_param<TY>(g.dgate, g.dgate_f32, at + row.col(j), dg[j]);
         }
       }
       if constexpr (POST) {
@@ -552,7 +600,7 @@ __global__ __launch_bounds__(block_of<TPR>(), TPR == 512 ? 4 : 1) void resnorm_b
         GRACE_EACH(dpw[j][i] = fmaf(S[j][i], phat[j][i], dpw[j][i]))
         if constexpr (BIAS) GRACE_EACH(dpb[j][i] += S[j][i])
         if (g.post_weight.p != nullptr) {
-          params.get(PW, at_lds.at[kPw], p);
+          params.template get<TY>(PW, places.at[kPw], row, g.post_weight, 0, p);
           GRACE_EACH(S[j][i] *= p[j][i])
         }
         GRACE_EACH(c1 += S[j][i]; c2 = fmaf(S[j][i], phat[j][i], c2))
@@ -565,8 +613,8 @@ __global__ __launch_bounds__(block_of<TPR>(), TPR == 512 ? 4 : 1) void resnorm_b
     }
     if constexpr (GATED) {
       if (g.dgate_mode == kGateGroups) {
-        over_slots(dg, row, red, [&](int c, const float(&v)[V], int k) {
-          store_param<TY>(g.dgate, g.dgate_f32, (int64_t)grp * n.d + c, v, k);
+        over_slots(dg, row, red, [&](int c, const float(&v)[V]) {
+          store_param<TY>(g.dgate, g.dgate_f32, (int64_t)grp * n.d + c, v);
         });
         GRACE_EACH(dg[j][i] = 0.f)
       }
@@ -576,7 +624,7 @@ __global__ __launch_bounds__(block_of<TPR>(), TPR == 512 ? 4 : 1) void resnorm_b
   auto leave = [&](int which, const float(&acc)[J][V]) {
     if (!g.want[which]) return;
     float* to = g.part + which * plane + blockIdx.x * (int64_t)n.d;
-    over_slots(acc, row, red, [&](int c, const float(&v)[V], int k) { store_vec(to + c, v, k); });
+    over_slots(acc, row, red, [&](int c, const float(&v)[V]) { store_vec(to + c, v); });
   };
   leave(kDw, dw);
   if constexpr (BIAS) leave(kDb, db);
@@ -588,11 +636,15 @@ __global__ __launch_bounds__(block_of<TPR>(), TPR == 512 ? 4 : 1) void resnorm_b
 }
 
 // ---------------------------------------------------------------- launches
-// Values per thread and threads per row, by the row's width.
+// Values per thread and threads per row, by the row's width.  Narrow rows share a wave by fours (64 bf16 columns,
+// forward and backward: 4.7 and 4.3 TB/s, with a wave for each row 0.9 and 1.6); more than 16 values to a thread
+// would spill, and a row is spread over no more waves than it needs, for each sum waits for all of them.
 template <typename F>
 void by_width(int d, F&& f) {
   using std::integral_constant;
-  if (d <= 64 * 8) f(integral_constant<int, 8>{}, integral_constant<int, 64>{});
+  if (d <= 16 * 8) f(integral_constant<int, 8>{}, integral_constant<int, 16>{});
+  else if (d <= 16 * 16) f(integral_constant<int, 16>{}, integral_constant<int, 16>{});
+  else if (d <= 64 * 8) f(integral_constant<int, 8>{}, integral_constant<int, 64>{});
   else if (d <= 64 * 16) f(integral_constant<int, 16>{}, integral_constant<int, 64>{});
   else if (d <= 256 * 8) f(integral_constant<int, 8>{}, integral_constant<int, 256>{});
   else if (d <= 512 * 8) f(integral_constant<int, 8>{}, integral_constant<int, 512>{});
@@ -631,38 +683,46 @@ unsigned resident(int block, unsigned lds) {
 
 template <typename TX, typename TY>
 void launch_forward(const FwdArgs& a, hipStream_t stream) {
-  by_width(a.n.d, [&](auto e, auto tpr) {
-    constexpr int E = decltype(e)::value, TPR = decltype(tpr)::value, B = block_of<TPR>();
+  auto launch = [&](auto e, auto tpr, auto v) {
+    constexpr int E = decltype(e)::value, TPR = decltype(tpr)::value, V = decltype(v)::value, B = block_of<TPR>();
+    constexpr auto kernel = resnorm_fwd_kernel<TX, TY, E, TPR, V>;
     const ParamPlaces places(a.weight.p, a.bias.p, a.gate.p, a.n.post ? a.post_weight.p : nullptr,
                              a.n.post ? a.post_bias.p : nullptr);
-    constexpr int V = vec_of<TX, TY>();
-    const unsigned lds = places.n * Params<1, TPR, V, E / V, lds_forward<E, TPR>()>::kFloats * 4;
-    allow_lds<resnorm_fwd_kernel<TX, TY, E, TPR>>(lds);
+    const unsigned lds = places.n * Params<1, TPR, V, E / V, forward_home<TPR>()>::kFloats * 4;
+    allow_lds<kernel>(lds);
     // a last, half-empty round of workgroups would cost as much as a full one
-    const unsigned grid = (unsigned)std::min<int64_t>((a.n.rows + B / TPR - 1) / (B / TPR),
-                                                      resident<resnorm_fwd_kernel<TX, TY, E, TPR>>(B, lds));
-    resnorm_fwd_kernel<TX, TY, E, TPR><<<grid, B, lds, stream>>>(a);
+    const unsigned grid =
+        (unsigned)std::min<int64_t>((a.n.rows + B / TPR - 1) / (B / TPR), resident<kernel>(B, lds));
+    kernel<<<grid, B, lds, stream>>>(a);
+  };
+  by_width(a.n.d, [&](auto e, auto tpr) {
+    if (a.n.d % vec_of<TY>() == 0) launch(e, tpr, std::integral_constant<int, vec_of<TY>()>{});
+    else launch(e, tpr, std::integral_constant<int, 1>{});
   });
 }
 
 template <typename TX, typename TY>
 void launch_backward(const BwdArgs& a, hipStream_t stream) {
-  const bool bias = a.want[kDb] || a.want[kDpb] || a.post_bias.p != nullptr;
-  auto choose = [&](auto post, auto gated, auto biased) {
+  const bool whole = a.n.d % vec_of<TY>() == 0;
+  const bool bias = !whole || a.want[kDb] || a.want[kDpb] || a.post_bias.p != nullptr;
+  auto choose = [&](auto post, auto gated, auto biased, auto v) {
     constexpr bool POST = decltype(post)::value, GATED = decltype(gated)::value, BIAS = decltype(biased)::value;
+    constexpr int V = decltype(v)::value;
     by_width(a.n.d, [&](auto e, auto tpr) {
-      constexpr int E = decltype(e)::value, TPR = decltype(tpr)::value, V = vec_of<TX, TY>();
+      constexpr int E = decltype(e)::value, TPR = decltype(tpr)::value;
+      constexpr auto kernel = resnorm_bwd_kernel<TX, TY, E, TPR, V, POST, GATED, BIAS>;
       const ParamPlaces places(a.weight.p, nullptr, a.gate.p, POST ? a.post_weight.p : nullptr,
                                POST && BIAS ? a.post_bias.p : nullptr);
-      const unsigned lds = places.n * Params<1, TPR, V, E / V, lds_backward<E, TPR>()>::kFloats * 4;
-      allow_lds<resnorm_bwd_kernel<TX, TY, E, TPR, POST, GATED, BIAS>>(lds);
-      resnorm_bwd_kernel<TX, TY, E, TPR, POST, GATED, BIAS>
-          <<<(unsigned)a.split.blocks, block_of<TPR>(), lds, stream>>>(a);
+      const unsigned lds = places.n * Params<1, TPR, V, E / V, backward_home<E, TPR>()>::kFloats * 4;
+      allow_lds<kernel>(lds);
+      kernel<<<(unsigned)a.split.blocks, block_of<TPR>(), lds, stream>>>(a);
     });
   };
   auto by_bias = [&](auto post, auto gated) {
-    if (bias) choose(post, gated, std::true_type{});
-    else choose(post, gated, std::false_type{});
+    constexpr std::integral_constant<int, vec_of<TY>()> wide{};
+    if (!whole) choose(post, gated, std::true_type{}, std::integral_constant<int, 1>{});
+    else if (bias) choose(post, gated, std::true_type{}, wide);
+    else choose(post, gated, std::false_type{}, wide);
   };
   auto by_gate = [&](auto post) {
     if (a.gate.p != nullptr) by_bias(post, std::true_type{});

@@ -24,19 +24,23 @@ struct __attribute__((packed, aligned(sizeof(T)))) Pack {
 };
 
 // The same address, as a value of its own.  The element-wise branch of a partial vector works on it: seeing
-// one address in both branches, the compiler takes the elements they share out of the wide access, which
-// then falls apart into a halfword, two dwords and so on.
+// one address in both branches, the compiler takes the elements they share out of the wide access, which then
+// falls apart into a halfword, two dwords and so on.  It names global memory, which the compiler no longer
+// sees: a generic access in one branch would make every wait behind it one for all loads.
 template <typename T>
-__device__ __forceinline__ T* apart(T* p) {
-  asm("" : "+v"(p));
-  return p;
+using GlobalPtr = __attribute__((address_space(1))) T*;
+template <typename T>
+__device__ __forceinline__ GlobalPtr<T> apart(T* p) {
+  GlobalPtr<T> q = (GlobalPtr<T>)p;
+  asm("" : "+v"(q));
+  return q;
 }
 
 // V elements as stored, in whole registers (two 16-bit values to a register: a struct of elements that
 // lives across a loop gets a register for each)
 template <typename T, int V>
 struct Bits {
-  static constexpr int W = V * (int)sizeof(T) / 4;
+  static constexpr int W = (V * (int)sizeof(T) + 3) / 4;
   uint32_t w[W];
 };
 template <int W, int A>
@@ -44,11 +48,13 @@ struct __attribute__((packed, aligned(A))) Words {
   uint32_t w[W];
 };
 
-// the first n of V elements at p; the others are zero.  ONCE: data that passes the caches by (nontemporal)
+// The first n (1 or more) of V elements at p; the others are zero.  ONCE: data that passes the caches by (nontemporal)
 template <bool ONCE = false, typename T, int V>
-__device__ __forceinline__ void load_bits(const T* __restrict__ p, Bits<T, V>& o, int n) {
+__device__ __forceinline__ void load_bits(const T* __restrict__ p, Bits<T, V>& o, int n = V) {
   constexpr int W = Bits<T, V>::W;
-  if (n >= V) {
+  if constexpr (V == 1 && sizeof(T) == 2) {
+    o.w[0] = *reinterpret_cast<const uint16_t*>(p);
+  } else if (n >= V) {
     if constexpr (ONCE) {
       typedef uint32_t word __attribute__((aligned(2)));
 #pragma unroll
@@ -61,12 +67,12 @@ __device__ __forceinline__ void load_bits(const T* __restrict__ p, Bits<T, V>& o
   } else {
 #pragma unroll
     for (int i = 0; i < W; ++i) o.w[i] = 0;
-    const T* q = apart(p);
+    const GlobalPtr<const T> q = apart(p);
 #pragma unroll
     for (int i = 0; i < V; ++i) {
       if (i >= n) continue;
-      if constexpr (sizeof(T) == 4) o.w[i] = reinterpret_cast<const uint32_t*>(q)[i];
-      else o.w[i / 2] |= (uint32_t) reinterpret_cast<const uint16_t*>(q)[i] << (16 * (i & 1));
+      if constexpr (sizeof(T) == 4) o.w[i] = ((GlobalPtr<const uint32_t>)q)[i];
+      else o.w[i / 2] |= (uint32_t)((GlobalPtr<const uint16_t>)q)[i] << (16 * (i & 1));
     }
   }
 }
@@ -87,7 +93,7 @@ __device__ __forceinline__ void load_vec(const T* __restrict__ p, float (&o)[V],
 #pragma unroll
     for (int i = 0; i < V; ++i) o[i] = (float)r.v[i];
   } else {
-    const T* q = apart(p);
+    const GlobalPtr<const T> q = apart(p);
 #pragma unroll
     for (int i = 0; i < V; ++i) o[i] = i < n ? (float)q[i] : 0.f;
   }
@@ -110,7 +116,7 @@ __device__ __forceinline__ void store_vec(T* __restrict__ p, const float (&x)[V]
     }
     *reinterpret_cast<Pack<T, V>*>(p) = r;
   } else {
-    T* q = apart(p);
+    const GlobalPtr<T> q = apart(p);
 #pragma unroll
     for (int i = 0; i < V; ++i)
       if (i < n) q[i] = (T)x[i];

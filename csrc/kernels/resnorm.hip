@@ -70,8 +70,8 @@ __global__ __launch_bounds__(1024) void resnorm_fold_kernel(FoldArgs a) {
   if (w == 0 && at < a.d) {
 #pragma unroll
     for (int i = 1; i < 16; ++i) s += red[i][col];
-    const float o[1] = {s};
-    store_param<TY>(a.out[k], a.f32[k], row * a.d + at, o, 1);
+    if (a.f32[k]) static_cast<float*>(a.out[k])[row * a.d + at] = s;
+    else static_cast<TY*>(a.out[k])[row * a.d + at] = (TY)s;
   }
 }
 
