@@ -18,7 +18,8 @@ struct EmbedIds {
   int64_t pad;  // row without a gradient, or -1
 };
 
-constexpr int64_t kEmbedMaxWidth = 1 << 23;  // slabs of columns are a grid's second dimension
+// slabs of columns are a grid's second dimension, or a factor of its first, which holds less than 2^32 threads
+constexpr int64_t kEmbedMaxWidth = 1 << 21;
 
 // out[t, :] = round(scale * w[ids[t], :]); rows of w are w_stride elements apart
 void embed_forward(const EmbedIds& ids, const void* w, ElType tw, int64_t w_stride, int64_t d, float scale, void* out,

@@ -555,7 +555,8 @@ __global__ __launch_bounds__(block_of<TPR>(), TPR == 512 ? 4 : 1) void resnorm_b
       GRACE_EACH(phat[j][i] = bits_at(ry.v[j], i); hat[j][i] = bits_at(rs.v[j], i); S[j][i] = bits_at(rdh.v[j], i);
                  ds[j][i] = bits_at(rds.v[j], i))
       if (AHEAD && r + kSlots < r_end) fetch(r + kSlots);
-      if constexpr (POST) GRACE_EACH(phat[j][i] = (phat[j][i] - pmean) * prstd)
+      // outside the width everything stays zero: a large mean there would make an infinity of zero, and NaN of the sums
+      if constexpr (POST) GRACE_EACH(phat[j][i] = (phat[j][i] - (row.in(j) ? pmean : 0.f)) * prstd)
       if (again) {
         float u[J][V];
         made_u(u);
@@ -565,7 +566,7 @@ __global__ __launch_bounds__(block_of<TPR>(), TPR == 512 ? 4 : 1) void resnorm_b
         }
         GRACE_EACH(hat[j][i] = fmaf(n.alpha, hat[j][i], u[j][i]))
       }
-      GRACE_EACH(hat[j][i] = (hat[j][i] - mean) * rstd; dw[j][i] = fmaf(S[j][i], hat[j][i], dw[j][i]))
+      GRACE_EACH(hat[j][i] = (hat[j][i] - (row.in(j) ? mean : 0.f)) * rstd; dw[j][i] = fmaf(S[j][i], hat[j][i], dw[j][i]))
       if constexpr (BIAS) GRACE_EACH(db[j][i] += S[j][i])
       if (g.weight.p != nullptr) {
         params.template get<TY>(W, places.at[kW], row, g.weight, 0, p);

@@ -44,7 +44,7 @@ __global__ __launch_bounds__(kBlock) void embed_fwd_kernel(EmbedIds ids, const T
                                                            int lanes_log) {
   constexpr int V = vec_of<TW, TO>(), kSteps = 2;
   const int lanes = 1 << lanes_log, lane = threadIdx.x & (lanes - 1);
-  const int64_t t = ((int64_t)blockIdx.x * kBlock + threadIdx.x) >> lanes_log;
+  const int64_t t = (((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * kBlock + threadIdx.x) >> lanes_log;
   if (t >= ids.n) return;
   const int64_t id = id_at(ids, t);
   const bool ok = id >= 0 && id < ids.vocab;
@@ -557,7 +557,9 @@ void embed_forward(const EmbedIds& ids, const void* w, ElType tw, int64_t w_stri
       using TO = std::remove_pointer_t<decltype(tag_o)>;
       int log = 0;
       while (log < 6 && ((int64_t)vec_of<TW, TO>() << log) < d) ++log;
-      const unsigned grid = (unsigned)cdiv(ids.n << log, kBlock);
+      // a dimension of a grid holds less than 2^32 threads
+      const int64_t blocks = cdiv(ids.n << log, kBlock), x = std::min<int64_t>(blocks, 1 << 23);
+      const dim3 grid((unsigned)x, (unsigned)cdiv(blocks, x));
       embed_fwd_kernel<TW, TO><<<grid, kBlock, 0, stream>>>(ids, (const TW*)w, w_stride, d, scale, (TO*)out, log);
     });
   });

@@ -1,5 +1,6 @@
 // Python bindings for the language-model training kernels (csrc/include/grace_lm.h): embedding,
 // residual norms, the global gradient norm.
+#include <torch/csrc/autograd/functions/accumulate_grad.h>
 #include <torch/extension.h>
 #include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
@@ -84,6 +85,27 @@ void once_only(const char* what) {
   TORCH_CHECK(!at::GradMode::is_enabled(), what, " is differentiable once: no create_graph");
 }
 
+// A backward that is captured into a graph reaches its leaves on the stream where autograd met them first; an
+// eager graph that is still alive keeps that.  If it is the default stream, which no capture can join, the
+// process would end: refused while nothing is recorded for the leaf.
+void no_foreign_leaf(const char* what) {
+  const hipStream_t stream = cur_stream();
+  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+  if (hipStreamIsCapturing(stream, &status) != hipSuccess) {
+    (void)hipGetLastError();
+    return;
+  }
+  const auto node = torch::autograd::get_current_node();
+  if (status == hipStreamCaptureStatusNone || node == nullptr) return;
+  for (const auto& edge : node->next_edges()) {
+    const auto* leaf = dynamic_cast<torch::autograd::AccumulateGrad*>(edge.function.get());
+    if (leaf == nullptr) continue;
+    const auto of = edge.function->stream();
+    TORCH_CHECK(!of.has_value() || of->id() != 0, what, ": a captured backward reaches a leaf that an eager graph on "
+                "the default stream still holds; let go of that graph's outputs first, or run it on another stream");
+  }
+}
+
 // A call that autograd does not follow would lose forward-mode tangents without a word.
 void no_tangent(const Tensor& t, const char* what) {
   TORCH_CHECK_NOT_IMPLEMENTED(!t._fw_grad(0).defined(), what, " has no forward-mode derivative");
@@ -100,6 +122,7 @@ struct EmbeddingFn : torch::autograd::Function<EmbeddingFn> {
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
                                                  torch::autograd::variable_list grads) {
     once_only("embedding");
+    no_foreign_leaf("embedding");
     const Tensor ids = ctx->get_saved_variables()[0];
     const auto args = ctx->saved_data["args"].toIntVector();
     return {embed_bwd(ids, grads[0].contiguous(), args[0], args[1], ctx->saved_data["scale"].toDouble(),
@@ -280,6 +303,7 @@ struct ResidualNormFn : torch::autograd::Function<ResidualNormFn> {
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
                                                  torch::autograd::variable_list grads) {
     once_only("residual norm");
+    no_foreign_leaf("residual norm");
     torch::autograd::variable_list out(9);
     const Tensor dh = grads[0].defined() ? grads[0].contiguous() : Tensor();
     const Tensor ds = grads.size() > 1 && grads[1].defined() ? grads[1].contiguous() : Tensor();

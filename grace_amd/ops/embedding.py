@@ -24,7 +24,7 @@ def embedding(ids: torch.Tensor, weight: torch.Tensor, scale: float = 1.0, paddi
     """``round(scale * weight[ids])`` of shape ``[*ids.shape, width]``.
 
     ``ids``: int64 or int32, any shape and strides.  ``weight``: ``[rows, width]``, float32, bfloat16 or
-    float16.  ``dtype``: the output's type (default: the table's).  ``padding_idx`` (negative: from the end)
+    float16, on a GPU at most 2^21 wide.  ``dtype``: the output's type (default: the table's).  ``padding_idx`` (negative: from the end)
     names a row that gets no gradient.  Differentiable once, in ``weight``."""
     if _native.use_native(weight):
         return _native.lib().embedding(ids, weight, scale, padding_idx, dtype)  # the same refusals, in C++

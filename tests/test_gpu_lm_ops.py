@@ -92,6 +92,8 @@ def test_embedding_layouts():
         embedding(ids, w.double())
     with pytest.raises(ValueError):
         embedding(ids.cpu(), w)
+    with pytest.raises(ValueError):
+        embedding(ids, torch.empty(40, 1, device="cuda").expand(40, 2**21 + 1))
 
 
 def test_embedding_far_rows():
@@ -107,6 +109,16 @@ def test_embedding_far_rows():
     assert torch.equal(dw[2**20 + 4], (dy[0].float() + dy[2].float()).bfloat16())
     assert torch.equal(dw[3], dy[1]) and torch.equal(dw[2**20], dy[3])
     assert int(dw.any(1).sum()) == 3
+
+
+def test_embedding_many_tokens():
+    """More threads than a dimension of a grid takes: 2^26 wave-wide rows and some."""
+    n = 2**26 + 77
+    w = torch.randn(3, 260, device="cuda").bfloat16()
+    ids = torch.arange(n, device="cuda", dtype=torch.int32) % 3
+    y = embedding(ids, w)
+    for at in (0, 2**25 - 5, 2**26 - 5, n - 60):
+        assert torch.equal(y[at:at + 60], w[ids[at:at + 60]])
 
 
 # ---------------------------------------------------------------------------- residual norm
@@ -188,6 +200,26 @@ def test_residual_norm_special_values():
         residual_norm(torch.zeros(1, 16385, device="cuda"))
     with pytest.raises(TypeError):
         residual_norm(torch.zeros(1, 4, device="cuda", dtype=F64))
+
+
+@pytest.mark.parametrize("t", [F32, BF16])
+@pytest.mark.parametrize("d", [96, 651, 1100, 4099])
+@pytest.mark.parametrize("post", [False, True])
+def test_residual_norm_of_a_large_constant(d, t, post):
+    """mean / deviation overflows fp32, but no value of the row has it: h = 0 and
+    dy = r (dh - mean dh), once for each norm, with r = 1 / sqrt(eps)."""
+    y = torch.full((3, d), 2.0**110, dtype=t, device="cuda", requires_grad=True)  # the sums over the row are exact
+    w = torch.ones(d, device="cuda", requires_grad=True)
+    g = torch.Generator("cuda").manual_seed(d)
+    dh = torch.randn(3, d, device="cuda", generator=g).to(t)
+    h = residual_norm(y, None, w, eps=1e-12, post=post)
+    assert not h.any()
+    dy, dw = torch.autograd.grad(h, [y, w], dh)
+    assert not dw.any()
+    r = 1e6 ** (1 + post)
+    a = dh.double()
+    mass = a.abs() + a.abs().mean(1, keepdim=True)
+    O.within(dy, r * (a - a.mean(1, keepdim=True)), 2 * O.K * O.U * r * mass)
 
 
 @pytest.mark.parametrize("tx,ty", [(F32, F32), (BF16, BF16), (F32, F16)])
@@ -419,6 +451,32 @@ def test_operators_in_a_graph():
         for _, outs in graphs:
             for a, e in zip(outs, want):
                 assert torch.equal(a, e)
+
+
+def test_captured_backward_beside_an_eager_graph():
+    """An eager graph on the default stream that holds a leaf: the captured backward is refused, and runs without it."""
+    ids = torch.arange(40, device="cuda") % 7
+    w = torch.randn(7, 24, device="cuda", requires_grad=True)
+    y = torch.randn(40, 24, device="cuda", requires_grad=True)
+    dy = torch.randn(40, 24, device="cuda")
+    for f, leaf in ((lambda: embedding(ids, w), w), (lambda: residual_norm(y), y)):
+        eager = f()
+        want, = torch.autograd.grad(eager, leaf, dy, retain_graph=True)
+        torch.cuda.synchronize()
+        with pytest.raises(RuntimeError, match="eager graph"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                torch.autograd.grad(f(), leaf, dy)
+        torch.cuda.synchronize()
+        assert torch.equal(torch.autograd.grad(eager, leaf, dy)[0], want)
+        del eager
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got, = torch.autograd.grad(f(), leaf, dy)
+        for _ in range(3):
+            got.zero_()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(got, want)
 
 
 def test_operators_on_another_stream():
