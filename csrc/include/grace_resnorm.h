@@ -21,9 +21,8 @@
 // partial row; a second launch adds the partial rows in a fixed order.
 //
 // Bound by memory: a copy runs at 5.2 TB/s.  64 million values in whole vectors, forward and backward: bf16 widths of
-// 256 to 8192 at 5.0-5.6 and 4.2-4.4 TB/s, fp32 at 4.6-5.5 and 4.6-4.9.  What does not reach that: a norm before and
-// behind with a gate keeps five sums and four weights a value, which 1024 threads of 128 registers do not hold
-// (backward, 12000 columns: 0.8 TB/s in bf16, 2.0 in fp32; up to 8192 columns 3.3-4.8).
+// 256 to 16384 at 4.9-5.6 and 4.1-4.5 TB/s, fp32 at 4.5-5.5 and 4.1-4.9.  With a norm behind the block and a gate: up
+// to 8192 columns 4.2-5.3 and 3.8-4.9, wider ones 3.8-4.2 and, for want of registers, 2.5 (bf16) and 4.2 (fp32).
 #pragma once
 
 #include <algorithm>
@@ -312,6 +311,43 @@ struct Params {
   }
 };
 
+// Column sums of a thread's own values, in registers or, where those are short, in LDS (places as Params').
+template <int TPR, int V, int J, bool LDS>
+struct ColumnSum {
+  using Lds = Params<1, TPR, V, J, kInLds>;
+  float r[LDS ? 1 : J][V];
+  Lds at;
+  __device__ __forceinline__ explicit ColumnSum(float* p) : at(p) { clear(); }
+  __device__ __forceinline__ void clear() { each([](float, int, int) { return 0.f; }); }
+  __device__ __forceinline__ void add(const float (&x)[J][V]) {
+    each([&](float a, int j, int i) { return a + x[j][i]; });
+  }
+  __device__ __forceinline__ void fma(const float (&x)[J][V], const float (&y)[J][V]) {
+    each([&](float a, int j, int i) { return fmaf(x[j][i], y[j][i], a); });
+  }
+  __device__ __forceinline__ void get(float (&v)[J][V]) {
+    each([&](float a, int j, int i) { return v[j][i] = a; });
+  }
+  template <typename F>
+  __device__ __forceinline__ void each(F&& f) {
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+      if constexpr (LDS) {
+#pragma unroll
+        for (int i = 0; i < V; i += Lds::kAccess) {
+          typename Lds::Part q = at.part(0, j, i);
+#pragma unroll
+          for (int m = 0; m < Lds::kAccess; ++m) q.v[m] = f(q.v[m], j, i + m);
+          at.part(0, j, i) = q;
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) r[j][i] = f(r[j][i], j, i);
+      }
+    }
+  }
+};
+
 // the workgroup's slot of rows; known to be the same in a wave where it is
 template <int TPR>
 __device__ __forceinline__ int row_slot() {
@@ -341,6 +377,12 @@ constexpr Home forward_home() { return TPR <= kWave ? kInMemory : TPR < 1024 ? k
 // Backward: at most four arrays in LDS, 128 KB.
 template <int E, int TPR>
 constexpr Home backward_home() { return TPR <= kWave ? kInRegisters : E == 8 ? kInLds : kInMemory; }
+
+// Rows of 16 values for each of 1024 threads with a post norm or a gate: two of the sums in LDS, 128 KB, for the
+// weights are not there.  All of them in 128 registers would spill: 12000 columns with both, backward,
+// 0.8 TB/s for 2.5 in bf16 and 2.0 for 4.2 in fp32.
+template <int E, int TPR, bool POST, bool GATED>
+constexpr bool sums_in_lds() { return backward_home<E, TPR>() == kInMemory && (POST || GATED); }
 
 #define GRACE_EACH(body)          \
   _Pragma("unroll") for (int j = 0; j < J; ++j) \
@@ -470,9 +512,10 @@ __device__ __forceinline__ void over_slots(const float (&acc)[J][V], const Row<T
   }
 }
 
-// BIAS: one of the two biases is there
+// BIAS: one of the two biases is there.  Four waves to a SIMD hold 128 registers each: a few of them spilled cost less
+// than the fourth wave (fp32, 1536 columns, gate and post norm: 332 us, 362 us with three waves of 131 registers).
 template <typename TX, typename TY, int E, int TPR, int V, bool POST, bool GATED, bool BIAS>
-__global__ __launch_bounds__(block_of<TPR>(), TPR == 512 ? 4 : 1) void resnorm_bwd_kernel(BwdArgs g) {
+__global__ __launch_bounds__(block_of<TPR>(), TPR == 512 || (TPR == 256 && V > 1) ? 4 : 1) void resnorm_bwd_kernel(BwdArgs g) {
   constexpr int J = E / V, kSlots = block_of<TPR>() / TPR;
   // The next row's loads are issued before this row's sums, where registers hold them: 1024 threads have 128 each,
   // and a single 16-bit value takes as much of them as two in a vector.
@@ -483,9 +526,12 @@ __global__ __launch_bounds__(block_of<TPR>(), TPR == 512 ? 4 : 1) void resnorm_b
   RowSum<TPR> sum{scratch};
   const NormShape& n = g.n;
   const Row<TPR, V, J> row(threadIdx.x % TPR, n.d);
-  float dw[J][V], db[J][V], dg[J][V], dpw[J][V], dpb[J][V];
-  GRACE_EACH(dw[j][i] = db[j][i] = dg[j][i] = dpw[j][i] = dpb[j][i] = 0.f)
   extern __shared__ __align__(16) float dyn[];
+  constexpr bool kLds = sums_in_lds<E, TPR, POST, GATED>();
+  ColumnSum<TPR, V, J, kLds> dw(dyn);
+  ColumnSum<TPR, V, J, kLds && POST> dpw(dyn + TPR * E);
+  ColumnSum<TPR, V, J, kLds && !POST> dg(dyn + TPR * E);
+  ColumnSum<TPR, V, J, false> db(dyn), dpb(dyn);
   Params<2 + 2 * POST, TPR, V, J, backward_home<E, TPR>()> params(dyn);
   constexpr int W = 0, G = 1, PW = 2, PB = 3;  // the places in registers
   const ParamPlaces places(g.weight.p, nullptr, g.gate.p, POST ? g.post_weight.p : nullptr,
@@ -566,8 +612,9 @@ __global__ __launch_bounds__(block_of<TPR>(), TPR == 512 ? 4 : 1) void resnorm_b
         }
         GRACE_EACH(hat[j][i] = fmaf(n.alpha, hat[j][i], u[j][i]))
       }
-      GRACE_EACH(hat[j][i] = (hat[j][i] - (row.in(j) ? mean : 0.f)) * rstd; dw[j][i] = fmaf(S[j][i], hat[j][i], dw[j][i]))
-      if constexpr (BIAS) GRACE_EACH(db[j][i] += S[j][i])
+      GRACE_EACH(hat[j][i] = (hat[j][i] - (row.in(j) ? mean : 0.f)) * rstd)
+      dw.fma(S, hat);
+      if constexpr (BIAS) db.add(S);
       if (g.weight.p != nullptr) {
         params.template get<TY>(W, places.at[kW], row, g.weight, 0, p);
         GRACE_EACH(S[j][i] *= p[j][i])
@@ -588,18 +635,19 @@ __global__ __launch_bounds__(block_of<TPR>(), TPR == 512 ? 4 : 1) void resnorm_b
         float u[J][V];
         made_u(u);
         params.template get<TY>(G, places.at[kG], row, g.gate, (int64_t)gate_now * n.d, p);
-        GRACE_EACH(u[j][i] *= S[j][i]; dg[j][i] = g.dgate_mode == kGateRows ? u[j][i] : dg[j][i] + u[j][i];
-                   S[j][i] *= p[j][i])
+        GRACE_EACH(u[j][i] *= S[j][i]; S[j][i] *= p[j][i])
         if (g.dgate_mode == kGateRows) {
 #pragma unroll
           for (int j = 0; j < J; ++j)
-            if (row.in(j)) store_param<TY>(g.dgate, g.dgate_f32, at + row.col(j), dg[j]);
+            if (row.in(j)) store_param<TY>(g.dgate, g.dgate_f32, at + row.col(j), u[j]);
+        } else {
+          dg.add(u);
         }
       }
       if constexpr (POST) {
         c1 = c2 = 0.f;
-        GRACE_EACH(dpw[j][i] = fmaf(S[j][i], phat[j][i], dpw[j][i]))
-        if constexpr (BIAS) GRACE_EACH(dpb[j][i] += S[j][i])
+        dpw.fma(S, phat);
+        if constexpr (BIAS) dpb.add(S);
         if (g.post_weight.p != nullptr) {
           params.template get<TY>(PW, places.at[kPw], row, g.post_weight, 0, p);
           GRACE_EACH(S[j][i] *= p[j][i])
@@ -614,17 +662,21 @@ __global__ __launch_bounds__(block_of<TPR>(), TPR == 512 ? 4 : 1) void resnorm_b
     }
     if constexpr (GATED) {
       if (g.dgate_mode == kGateGroups) {
-        over_slots(dg, row, red, [&](int c, const float(&v)[V]) {
+        float v[J][V];
+        dg.get(v);
+        over_slots(v, row, red, [&](int c, const float(&v)[V]) {
           store_param<TY>(g.dgate, g.dgate_f32, (int64_t)grp * n.d + c, v);
         });
-        GRACE_EACH(dg[j][i] = 0.f)
+        dg.clear();
       }
     }
   }
   const int64_t plane = g.split.blocks * n.d;
-  auto leave = [&](int which, const float(&acc)[J][V]) {
+  auto leave = [&](int which, auto& sum) {
     if (!g.want[which]) return;
     float* to = g.part + which * plane + blockIdx.x * (int64_t)n.d;
+    float acc[J][V];
+    sum.get(acc);
     over_slots(acc, row, red, [&](int c, const float(&v)[V]) { store_vec(to + c, v); });
   };
   leave(kDw, dw);
@@ -714,7 +766,9 @@ void launch_backward(const BwdArgs& a, hipStream_t stream) {
       constexpr auto kernel = resnorm_bwd_kernel<TX, TY, E, TPR, V, POST, GATED, BIAS>;
       const ParamPlaces places(a.weight.p, nullptr, a.gate.p, POST ? a.post_weight.p : nullptr,
                                POST && BIAS ? a.post_bias.p : nullptr);
-      const unsigned lds = places.n * Params<1, TPR, V, E / V, backward_home<E, TPR>()>::kFloats * 4;
+      const unsigned lds = sums_in_lds<E, TPR, POST, GATED>()
+                               ? 2 * TPR * E * 4
+                               : places.n * Params<1, TPR, V, E / V, backward_home<E, TPR>()>::kFloats * 4;
       allow_lds<kernel>(lds);
       kernel<<<(unsigned)a.split.blocks, block_of<TPR>(), lds, stream>>>(a);
     });

@@ -126,6 +126,7 @@ NORM = [  # batch, length, width, residual, block
     (1, 1, 1, F32, F32), (1, 1, 7, BF16, BF16), (2, 3, 63, F32, F32), (4, 1, 768, BF16, BF16), (35, 21, 651, F16, F16),
     (3, 50, 768, F32, BF16), (2, 3, 1024, F32, F32), (2, 5, 1025, BF16, BF16), (1, 300, 33, F32, F16),
     (2, 9, 4096, BF16, BF16), (3, 3, 4099, F32, F32), (2, 3, 16384, BF16, BF16), (1, 2, 8191, F32, F32),
+    (2, 5, 9001, BF16, BF16), (1, 300, 9000, F32, F16), (2, 9, 12000, F32, F32),
     (1100, 2, 20, F32, F32), (7, 900, 12, BF16, BF16), (300, 30, 16, None, BF16), (5, 3, 130, None, F32)]
 
 
