@@ -15,7 +15,9 @@ namespace {
 
 using namespace resnorm;
 
-constexpr int kMinRows = 2;  // rows per row slot of a workgroup before another workgroup is added
+// Rows per row slot of a workgroup before another workgroup is added, where there is one for each CU: 4096 fp32 rows of
+// 768 take 11.1 + 3.9 us (backward and fold) with two and 12.8 + 5.0 us with one, 735 fp16 rows of 651 10.8 and 8.3 us.
+constexpr int kMinRows = 2;
 
 struct FoldArgs {
   const float* part;
@@ -92,7 +94,8 @@ Shape shape_of(int d) {
 
 Split split_rows(const NormShape& n, bool grouped) {
   const Shape shape = shape_of(n.d);
-  const int64_t most = std::max<int64_t>(1, std::min<int64_t>(shape.resident, cdiv(n.rows, (int64_t)shape.slots * kMinRows)));
+  const int64_t one = cdiv(n.rows, shape.slots), several = cdiv(n.rows, (int64_t)shape.slots * kMinRows);
+  const int64_t most = std::max<int64_t>(1, std::min<int64_t>(shape.resident, std::max(several, std::min<int64_t>(one, kCUs))));
   Split s{1, n.rows, most, 1, most};
   if (grouped && n.gate_rows < n.rows) {
     s.groups = n.rows / n.gate_rows;
@@ -105,8 +108,8 @@ Split split_rows(const NormShape& n, bool grouped) {
 }
 
 // A backward that moves more than twice the 256 MB memory-side cache stores past it, for what it writes first is
-// gone from there when it ends: 330 us for 346 us at 32768 bf16 rows of 4096.  (The forward loses by it:
-// 219 us for 205 us.)
+// gone from there when it ends: 64 million fp32 values in rows of 1024 take 214 us for 218 us, with gate and post
+// norm 316 for 327 (32768 bf16 rows of 4096: the same).  The forward loses by it: 219 us for 205 us there.
 bool moves_much(const NormShape& n) { return n.rows * n.d * (el_bytes(n.tx) + el_bytes(n.ty)) * 2 > (512ll << 20); }
 
 template <typename F>
