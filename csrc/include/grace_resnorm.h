@@ -21,8 +21,8 @@
 // partial row; a second launch adds the partial rows in a fixed order.
 //
 // Bound by memory: a copy runs at 5.2 TB/s.  64 million values in whole vectors, forward and backward: bf16 widths of
-// 256 to 16384 at 4.9-5.6 and 4.1-4.5 TB/s, fp32 at 4.5-5.5 and 4.1-4.9.  With a norm behind the block and a gate: up
-// to 8192 columns 4.2-5.3 and 3.8-4.9, wider ones 3.8-4.2 and, for want of registers, 2.5 (bf16) and 4.2 (fp32).
+// 64 to 16384 at 4.7-5.5 and 4.0-4.4 TB/s, fp32 at 4.7-5.5 and 4.1-4.9.  With a norm behind the block and a gate: up to
+// 8192 columns 4.4-5.5 and 3.1-4.9, wider ones 3.8-4.2 and, for want of registers, 2.5 (bf16) and 4.2 (fp32).
 #pragma once
 
 #include <algorithm>
@@ -41,11 +41,19 @@ template <int TPR>
 constexpr int block_of() { return TPR < 256 ? 256 : TPR; }
 
 // Values per load: 16 bytes of the narrower type where the rows are whole vectors.  A row that ends inside one is
-// taken by single values, so that a wave's accesses are aligned and next to each other: wide ones of 16-bit values at
-// odd addresses run at half the rate, and the branches of a partial vector cost registers and waits (bf16, forward
-// and backward: 1100 columns 3.6 and 2.8 TB/s, as vectors 2.3 and 2.4; 651 columns 4.1 and 3.7 for 3.5 and 3.8).
+// taken by single values, or pairs of 16 bits, so that a wave's accesses are aligned and next to each other: wide ones
+// of 16-bit values at odd addresses run at half the rate, and the branches of a partial vector cost registers and waits
+// (bf16, forward and backward: 1100 columns 3.8 and 4.2 TB/s as pairs, 3.6 and 2.8 as single values, 2.3 and 2.4 as
+// vectors; 651 columns 4.1 and 3.7 as single values, 3.5 and 3.8 as vectors).
 template <typename TY>
 constexpr int vec_of() { return sizeof(TY) == 2 ? 8 : 4; }
+template <typename TY, typename F>
+void by_vec(int d, F&& f) {
+  using std::integral_constant;
+  if (d % vec_of<TY>() == 0) f(integral_constant<int, vec_of<TY>()>{});
+  else if (sizeof(TY) == 2 && d % 2 == 0) f(integral_constant<int, sizeof(TY) == 2 ? 2 : 1>{});
+  else f(integral_constant<int, 1>{});
+}
 
 struct FwdArgs {
   NormShape n;
@@ -162,18 +170,18 @@ struct Row {
     for (int j = 0; j < J; ++j)
 #pragma unroll
       for (int i = 0; i < Bits<T, V>::W; ++i) r.v[j].w[i] = 0;
-    // asked once of 8 or 16 single values, but of every vector: two or four of them run better so
+    // asked once of 4 to 16 narrow accesses, but of every wide one: two or four of them run better so
     const bool there = p != nullptr;
-    if (V == 1 && !there) return;
+    if (V < 4 && !there) return;
 #pragma unroll
     for (int j = 0; j < J; ++j)
-      if ((V == 1 || there) && in(j)) load_bits(static_cast<const T*>(p) + at + col(j), r.v[j]);
+      if ((V < 4 || there) && in(j)) load_bits(static_cast<const T*>(p) + at + col(j), r.v[j]);
   }
-  // Before the first use of r: single 16-bit values are widened behind this, not where each is loaded, which would
+  // Before the first use of r: 16-bit values in narrow accesses are widened behind this, not where each is loaded, which would
   // make every load wait for the one before it.
   template <typename T>
   __device__ __forceinline__ void arrive(Raw<T, V, J>& r) const {
-    if constexpr (V == 1 && sizeof(T) == 2) {
+    if constexpr (V < 4 && sizeof(T) == 2) {
 #pragma unroll
       for (int j = 0; j < J; ++j) asm volatile("" : "+v"(r.v[j].w[0]));
     }
@@ -196,8 +204,8 @@ struct Row {
   }
   template <typename T>
   __device__ __forceinline__ void store(void* p, int64_t at, const float (&v)[J][V], bool once) const {
-    // single values leave lines in parts, for the cache to join (fp32, 130 columns: 280 us past it, 235 us through it)
-    if constexpr (V > 1) {
+    // narrow accesses leave lines in parts, for the cache to join (fp32, 130 columns: 280 us past it, 235 us through it)
+    if constexpr (V > 2) {
       if (once) {
 #pragma unroll
         for (int j = 0; j < J; ++j)
@@ -245,12 +253,16 @@ struct Row {
 };
 
 // Where the weights and the gate of a workgroup's rows are, each thread's own values of them.
-//   registers  rows of a wave or less
-//   LDS        rows of a workgroup, where they cost no registers: the registers decide how many such rows a CU has
-//              in flight.  Only the thread that wrote a value reads it, so there are no barriers.  An array
-//              takes 16 KB for rows of 512 threads and 8 values, 32 KB for 1024 threads.
-//   memory     rows of 16 values for each of 1024 threads, whose registers and LDS hold no more: from the caches
+//   registers  backward of rows of a wave or less, forward of rows of 1024 threads
+//   LDS        where they cost no registers: the registers decide how many rows a CU has in flight.  A thread reads
+//              what it wrote, or what the other row slots wrote to the same place, the same bits: no barriers.  An
+//              array takes 4 KB for rows of 64 threads and 16 values, 16 KB for 512 threads, 32 KB for 1024; the gate
+//              takes that for every row slot, for their rows may have different ones.
+//   memory     from the caches: backward of rows of 16 values for each of 1024 threads, whose registers and LDS hold no
+//              more, and forward of some rows of a wave
 enum Home { kInRegisters, kInLds, kInMemory };
+
+enum { kW, kB, kPw, kPb, kG, kParams };
 
 template <int K, int TPR, int V, int J, Home HOME>
 struct Params {
@@ -261,9 +273,11 @@ struct Params {
   };
   float r[HOME == kInRegisters ? K : 1][J][V];
   Part* lds;
-  __device__ __forceinline__ explicit Params(float* p) : lds(reinterpret_cast<Part*>(p) + threadIdx.x) {}
-  __device__ __forceinline__ Part& part(int place, int j, int i) const {
-    return lds[((place * J + j) * (V / kAccess) + i / kAccess) * TPR];
+  Part* own;  // the row slot's
+  __device__ __forceinline__ explicit Params(float* p)
+      : lds(reinterpret_cast<Part*>(p) + threadIdx.x % TPR), own(lds + threadIdx.x / TPR * (J * V / kAccess) * TPR) {}
+  __device__ __forceinline__ Part& part(int place, int j, int i, bool slot = false) const {
+    return (slot ? own : lds)[((place * J + j) * (V / kAccess) + i / kAccess) * TPR];
   }
   // k: the array (a constant), place: its place in LDS, from + at: where it is in memory
   template <typename TY>
@@ -279,7 +293,7 @@ struct Params {
 #pragma unroll
         for (int m = 0; m < kAccess; ++m) q.v[m] = v[j][i + m];
         if constexpr (HOME == kInLds) {
-          part(place, j, i) = q;
+          part(place, j, i, k == kG) = q;
         } else {
 #pragma unroll
           for (int m = 0; m < kAccess; ++m) r[k][j][i + m] = q.v[m];
@@ -290,8 +304,8 @@ struct Params {
   __device__ __forceinline__ void get(int k, int place, const Row<TPR, V, J>& row, const NormParam& from, int64_t at,
                                       float (&v)[J][V]) const {
     if constexpr (HOME == kInMemory) {
-      int64_t none = 0;  // which the compiler can't see: it would keep single values in registers, 16 for each array
-      if constexpr (V == 1) asm volatile("" : "+s"(none));
+      int64_t none = 0;  // which the compiler can't see: it would keep narrow ones in registers, 16 for each array
+      if constexpr (V < 4) asm volatile("" : "+s"(none));
       row.template param<TY>(from, at + none, v);
     } else {
 #pragma unroll
@@ -299,7 +313,7 @@ struct Params {
 #pragma unroll
         for (int i = 0; i < V; i += kAccess) {
           if constexpr (HOME == kInLds) {
-            const Part q = part(place, j, i);
+            const Part q = part(place, j, i, k == kG);
 #pragma unroll
             for (int m = 0; m < kAccess; ++m) v[j][i + m] = q.v[m];
           } else {
@@ -356,8 +370,6 @@ __device__ __forceinline__ int row_slot() {
   else return __builtin_amdgcn_readfirstlane(threadIdx.x / TPR);
 }
 
-enum { kW, kB, kPw, kPb, kG, kParams };
-
 // Which arrays there are, and their places in LDS (-1: not there).
 struct ParamPlaces {
   int at[kParams], n = 0;
@@ -369,11 +381,13 @@ struct ParamPlaces {
   }
 };
 
-// Forward: rows of a wave or less take the weights from the caches, so that few registers let many rows run at once
-// (16 values a thread and the weights in registers: 160 registers, two rounds for 4096 rows).  At most five
-// arrays in LDS, 80 KB; 1024 threads would take 160 KB and have registers enough.
-template <int TPR>
-constexpr Home forward_home() { return TPR <= kWave ? kInMemory : TPR < 1024 ? kInLds : kInRegisters; }
+// Forward: at most five arrays in LDS, 80 KB; 1024 threads would take 160 KB and have registers enough.  fp32 rows of 16
+// values a thread take them from the caches, when their sums are done: 4096 rows of 768 take 10.4 us and 11.3 with LDS,
+// which is filled before the first row; in 16 bits (64 million values in rows of 650) 3.6 TB/s and 4.4 with LDS.
+template <typename TY, int E, int TPR>
+constexpr Home forward_home() {
+  return TPR == 1024 ? kInRegisters : E == 16 && sizeof(TY) == 4 ? kInMemory : kInLds;
+}
 // Backward: at most four arrays in LDS, 128 KB.
 template <int E, int TPR>
 constexpr Home backward_home() { return TPR <= kWave ? kInRegisters : E == 8 ? kInLds : kInMemory; }
@@ -408,7 +422,7 @@ __global__ __launch_bounds__(block_of<TPR>()) void resnorm_fwd_kernel(FwdArgs g)
   };
   fetch(r);
   extern __shared__ __align__(16) float dyn[];
-  Params<kParams, TPR, V, J, forward_home<TPR>()> params(dyn);
+  Params<kParams, TPR, V, J, forward_home<TY, E, TPR>()> params(dyn);
   const ParamPlaces places(g.weight.p, g.bias.p, g.gate.p, n.post ? g.post_weight.p : nullptr,
                            n.post ? g.post_bias.p : nullptr);
   auto put = [&](int k, const NormParam& from) {
@@ -520,7 +534,7 @@ __global__ __launch_bounds__(block_of<TPR>(), TPR == 512 || (TPR == 256 && V > 1
   // The next row's loads are issued before this row's sums, where registers hold them: 1024 threads have 128 each,
   // and a single 16-bit value takes as much of them as two in a vector.
   constexpr bool AHEAD =
-      TPR > kWave && E == 8 && !(TPR == 1024 && sizeof(TY) == 4 && (POST || GATED)) && !(V == 1 && sizeof(TY) == 2);
+      TPR > kWave && E == 8 && !(TPR == 1024 && sizeof(TY) == 4 && (POST || GATED)) && !(V < (TPR == 1024 ? 4 : 2) && sizeof(TY) == 2);
   __shared__ float scratch[TPR > kWave ? 4 * TPR / kWave : 1];
   __shared__ float red[kSlots > 1 ? kSlots * TPR * E : 1];
   RowSum<TPR> sum{scratch};
@@ -741,7 +755,9 @@ void launch_forward(const FwdArgs& a, hipStream_t stream) {
     constexpr auto kernel = resnorm_fwd_kernel<TX, TY, E, TPR, V>;
     const ParamPlaces places(a.weight.p, a.bias.p, a.gate.p, a.n.post ? a.post_weight.p : nullptr,
                              a.n.post ? a.post_bias.p : nullptr);
-    const unsigned lds = places.n * Params<1, TPR, V, E / V, forward_home<TPR>()>::kFloats * 4;
+    // the gate's row is its row slot's own
+    const int arrays = places.n + (places.at[kG] >= 0 ? B / TPR - 1 : 0);
+    const unsigned lds = arrays * Params<1, TPR, V, E / V, forward_home<TY, E, TPR>()>::kFloats * 4;
     allow_lds<kernel>(lds);
     // a last, half-empty round of workgroups would cost as much as a full one
     const unsigned grid =
@@ -749,15 +765,13 @@ void launch_forward(const FwdArgs& a, hipStream_t stream) {
     kernel<<<grid, B, lds, stream>>>(a);
   };
   by_width(a.n.d, [&](auto e, auto tpr) {
-    if (a.n.d % vec_of<TY>() == 0) launch(e, tpr, std::integral_constant<int, vec_of<TY>()>{});
-    else launch(e, tpr, std::integral_constant<int, 1>{});
+    by_vec<TY>(a.n.d, [&](auto v) { launch(e, tpr, v); });
   });
 }
 
 template <typename TX, typename TY>
 void launch_backward(const BwdArgs& a, hipStream_t stream) {
-  const bool whole = a.n.d % vec_of<TY>() == 0;
-  const bool bias = !whole || a.want[kDb] || a.want[kDpb] || a.post_bias.p != nullptr;
+  const bool bias = a.want[kDb] || a.want[kDpb] || a.post_bias.p != nullptr;
   auto choose = [&](auto post, auto gated, auto biased, auto v) {
     constexpr bool POST = decltype(post)::value, GATED = decltype(gated)::value, BIAS = decltype(biased)::value;
     constexpr int V = decltype(v)::value;
@@ -774,10 +788,11 @@ void launch_backward(const BwdArgs& a, hipStream_t stream) {
     });
   };
   auto by_bias = [&](auto post, auto gated) {
-    constexpr std::integral_constant<int, vec_of<TY>()> wide{};
-    if (!whole) choose(post, gated, std::true_type{}, std::integral_constant<int, 1>{});
-    else if (bias) choose(post, gated, std::true_type{}, wide);
-    else choose(post, gated, std::false_type{}, wide);
+    by_vec<TY>(a.n.d, [&](auto v) {
+      if constexpr (decltype(v)::value == vec_of<TY>())
+        if (!bias) return choose(post, gated, std::false_type{}, v);
+      choose(post, gated, std::true_type{}, v);
+    });
   };
   auto by_gate = [&](auto post) {
     if (a.gate.p != nullptr) by_bias(post, std::true_type{});
