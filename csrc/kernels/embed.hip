@@ -37,7 +37,8 @@ constexpr int vec_of() { return sizeof(A) == 2 || sizeof(B) == 2 ? 8 : 4; }
 
 // ---------------------------------------------------------------- forward
 // 2^lanes_log lanes per token (a wave for wide rows, several tokens a wave for narrow ones), V columns per
-// lane and step; the loads of kSteps steps are under way before the first store.
+// lane and step; the loads of kSteps steps are under way before the first store.  Bound by memory: 65536 fp32 rows of
+// 1024 to bf16 take 47 us for at most 339 MB (frequent rows come from the caches); 8 bf16 rows of 768 2.2 us, a launch.
 template <typename TW, typename TO>
 __global__ __launch_bounds__(kBlock) void embed_fwd_kernel(EmbedIds ids, const TW* __restrict__ w, int64_t w_stride,
                                                            int64_t d, float scale, TO* __restrict__ out,
@@ -97,7 +98,8 @@ __device__ __forceinline__ void clear_rows(const EmbedIds& ids, int64_t r0, int6
 
 // Workgroup (token t, slab of columns), and behind those the ones that clear.  Each wave looks through a quarter of
 // the tokens and notes those of t's row; if t is the first of them the waves sum their notes and meet in LDS
-// in token order.
+// in token order.  700 tokens of 650 fp32 columns into 10000 rows: 12.6 us for 28 MB, the latency of a search, a sum and a
+// meeting one after the other (the sort's launches are four, and 25 us of the host's).
 template <typename TD, typename TG>
 __global__ __launch_bounds__(kBlock) void embed_few_kernel(EmbedIds ids, const TD* __restrict__ dy, int64_t d,
                                                            float scale, TG* __restrict__ dw, int slabs, int rows_each,
@@ -233,7 +235,8 @@ __device__ __forceinline__ void place(uint32_t (*hist)[kRadix], uint32_t base) {
   }
 }
 
-// n <= 1024 PER: workgroup 0 sorts, every pass in its LDS; the others clear dw.
+// n <= 1024 PER: workgroup 0 sorts, every pass in its LDS; the others clear dw.  4096 tokens, 15 bits: 14.6 us, in which
+// 94 MB are cleared at 6.4 TB/s (a fill alone reaches 6.8).
 template <int PER>
 __global__ __launch_bounds__(kSortBlock) void sort_small_kernel(EmbedIds ids, int bits, int passes,
                                                                 uint32_t* __restrict__ skey,
@@ -288,7 +291,8 @@ __global__ __launch_bounds__(kSortBlock) void sort_small_kernel(EmbedIds ids, in
 }
 
 // Digit counts of every tile of 1024 PER tokens, count[tile][digit]; the workgroups behind the tiles clear a
-// share of dw.  in = nullptr: the tokens themselves (the first pass).
+// share of dw.  in = nullptr: the tokens themselves (the first pass).  65536 tokens: 8.9 us and the move 10.7 us a pass;
+// both passes together clear 205 MB in 39 us, 5.2 TB/s.
 template <int PER>
 __global__ __launch_bounds__(kSortBlock) void sort_count_kernel(EmbedIds ids, int tiles,
                                                                 const uint32_t* __restrict__ in, int shift,
@@ -377,7 +381,7 @@ struct Runs {
   uint32_t* joins;      // their number, and then the chunks where such runs begin, in any order
 };
 
-// ONCE: nontemporal loads of dy.  134 MB of it take 39 us with them and 50 us without; what the caches can
+// Bound by memory.  ONCE: nontemporal loads of dy.  134 MB of it take 39 us with them and 50 us without; what the caches can
 // still hold from the pass that wrote it is read through them.
 constexpr int64_t kOnceBytes = 128ll << 20;
 template <typename TD, typename TG, bool ONCE>
@@ -447,7 +451,8 @@ __global__ __launch_bounds__(kBlock) void run_sum_kernel(Runs a, const TD* __res
 }
 
 // Adds up the partial rows of the runs that cross chunks, each in chunk order: the workgroup's waves take
-// every kJoinWaves-th partial row and meet in LDS.
+// every kJoinWaves-th partial row and meet in LDS.  An eighth of 65536 tokens the same, 1024 columns: 9.6 us, 4096 tokens
+// 4.8 us, bound by the latency of a search and two loads.
 constexpr int kJoinWaves = 8, kJoinBlocks = 1024;
 template <typename TG>
 __global__ __launch_bounds__(kJoinWaves* kWave) void run_join_kernel(Runs a, int64_t d, float scale,

