@@ -177,8 +177,8 @@ struct Row {
     for (int j = 0; j < J; ++j)
       if ((V < 4 || there) && in(j)) load_bits(static_cast<const T*>(p) + at + col(j), r.v[j]);
   }
-  // Before the first use of r: 16-bit values in narrow accesses are widened behind this, not where each is loaded, which would
-  // make every load wait for the one before it.
+  // Before the first use of r: 16-bit values in narrow accesses are widened behind this, not where each is loaded, which
+  // would make every load wait for the one before it.
   template <typename T>
   __device__ __forceinline__ void arrive(Raw<T, V, J>& r) const {
     if constexpr (V < 4 && sizeof(T) == 2) {
@@ -529,12 +529,13 @@ __device__ __forceinline__ void over_slots(const float (&acc)[J][V], const Row<T
 // BIAS: one of the two biases is there.  Four waves to a SIMD hold 128 registers each: a few of them spilled cost less
 // than the fourth wave (fp32, 1536 columns, gate and post norm: 332 us, 362 us with three waves of 131 registers).
 template <typename TX, typename TY, int E, int TPR, int V, bool POST, bool GATED, bool BIAS>
-__global__ __launch_bounds__(block_of<TPR>(), TPR == 512 || (TPR == 256 && V > 1) ? 4 : 1) void resnorm_bwd_kernel(BwdArgs g) {
+__global__ __launch_bounds__(block_of<TPR>(),
+                             TPR == 512 || (TPR == 256 && V > 1) ? 4 : 1) void resnorm_bwd_kernel(BwdArgs g) {
   constexpr int J = E / V, kSlots = block_of<TPR>() / TPR;
-  // The next row's loads are issued before this row's sums, where registers hold them: 1024 threads have 128 each,
-  // and a single 16-bit value takes as much of them as two in a vector.
-  constexpr bool AHEAD =
-      TPR > kWave && E == 8 && !(TPR == 1024 && sizeof(TY) == 4 && (POST || GATED)) && !(V < (TPR == 1024 ? 4 : 2) && sizeof(TY) == 2);
+  // The next row's loads are issued before this row's sums, where registers hold them: 1024 threads have 128 each, and a
+  // single 16-bit value takes as much of them as two in a vector.
+  constexpr bool kShort = sizeof(TY) == 2 ? V < (TPR == 1024 ? 4 : 2) : TPR == 1024 && (POST || GATED);
+  constexpr bool AHEAD = TPR > kWave && E == 8 && !kShort;
   __shared__ float scratch[TPR > kWave ? 4 * TPR / kWave : 1];
   __shared__ float red[kSlots > 1 ? kSlots * TPR * E : 1];
   RowSum<TPR> sum{scratch};
@@ -732,19 +733,19 @@ void allow_lds(unsigned bytes) {
     done.fetch_or(1ull << dev, std::memory_order_relaxed);
 }
 
-// Workgroups of a kernel that the chip holds at a time.
+// Workgroups of a kernel with so many arrays in LDS that the chip holds at a time; asked for once.
 template <auto Kernel>
-unsigned resident(int block, unsigned lds) {
-  static std::atomic<uint64_t> last{0};  // lds + 1 in the upper half, the answer in the lower
-  const uint64_t key = (uint64_t)lds + 1, known = last.load(std::memory_order_relaxed);
-  if (known >> 32 == key) return (unsigned)known;
+unsigned resident(int block, int arrays, unsigned lds) {
+  static std::atomic<unsigned> known[kParams + 16];
+  unsigned n = known[arrays].load(std::memory_order_relaxed);
+  if (n > 0) return n;
   int per_cu = 0;
   if (hipOccupancyMaxActiveBlocksPerMultiprocessor(&per_cu, Kernel, block, lds) != hipSuccess || per_cu < 1) {
     (void)hipGetLastError();
     per_cu = 1;
   }
-  const unsigned n = (unsigned)per_cu * kCUs;
-  last.store(key << 32 | n, std::memory_order_relaxed);
+  n = (unsigned)per_cu * kCUs;
+  known[arrays].store(n, std::memory_order_relaxed);
   return n;
 }
 
@@ -761,7 +762,7 @@ void launch_forward(const FwdArgs& a, hipStream_t stream) {
     allow_lds<kernel>(lds);
     // a last, half-empty round of workgroups would cost as much as a full one
     const unsigned grid =
-        (unsigned)std::min<int64_t>((a.n.rows + B / TPR - 1) / (B / TPR), resident<kernel>(B, lds));
+        (unsigned)std::min<int64_t>((a.n.rows + B / TPR - 1) / (B / TPR), resident<kernel>(B, arrays, lds));
     kernel<<<grid, B, lds, stream>>>(a);
   };
   by_width(a.n.d, [&](auto e, auto tpr) {

@@ -98,8 +98,8 @@ __device__ __forceinline__ void clear_rows(const EmbedIds& ids, int64_t r0, int6
 
 // Workgroup (token t, slab of columns), and behind those the ones that clear.  Each wave looks through a quarter of
 // the tokens and notes those of t's row; if t is the first of them the waves sum their notes and meet in LDS
-// in token order.  700 tokens of 650 fp32 columns into 10000 rows: 12.6 us for 28 MB, the latency of a search, a sum and a
-// meeting one after the other (the sort's launches are four, and 25 us of the host's).
+// in token order.  700 tokens of 650 fp32 columns into 10000 rows: 12.6 us for 28 MB, the latency of a search, a sum
+// and a meeting one after the other (sorting takes three launches).
 template <typename TD, typename TG>
 __global__ __launch_bounds__(kBlock) void embed_few_kernel(EmbedIds ids, const TD* __restrict__ dy, int64_t d,
                                                            float scale, TG* __restrict__ dw, int slabs, int rows_each,
@@ -381,8 +381,8 @@ struct Runs {
   uint32_t* joins;      // their number, and then the chunks where such runs begin, in any order
 };
 
-// Bound by memory.  ONCE: nontemporal loads of dy.  134 MB of it take 39 us with them and 50 us without; what the caches can
-// still hold from the pass that wrote it is read through them.
+// Bound by memory.  ONCE: nontemporal loads of dy.  134 MB of it take 39 us with them and 50 us without; what the
+// caches can still hold from the pass that wrote it is read through them.
 constexpr int64_t kOnceBytes = 128ll << 20;
 template <typename TD, typename TG, bool ONCE>
 __global__ __launch_bounds__(kBlock) void run_sum_kernel(Runs a, const TD* __restrict__ dy, int64_t d, float scale,

@@ -32,7 +32,7 @@ struct FoldArgs {
 
 // One workgroup adds 64 columns of one output row.  16 lanes read the columns of a partial row, so the
 // workgroup's 64 slices have 64 x kAhead rows in flight: the launch is one or two latencies long (3.9 us for 512
-// partial rows of two sums of 768 columns, 9 us for 1024 of three of 4096).
+// partial rows of two sums of 768 columns, 9 us for 512 of three of 4096).
 constexpr int kFoldCols = 64, kFoldSlices = 64, kAhead = 4;
 template <typename TY>
 __global__ __launch_bounds__(1024) void resnorm_fold_kernel(FoldArgs a) {
