@@ -168,6 +168,28 @@ def test_residual_norm_layouts():
     norm_case(v, dh[:1, :1].expand(6, 10, 40), ds, "rms", 1.0, False)
 
 
+@pytest.mark.parametrize("d", [24, 64, 130, 200, 650, 651, 2050])
+def test_residual_norm_16_bit_views(d):
+    """Every tensor, weights too, one element behind an aligned address; many gates in a workgroup."""
+    v, dh, ds = norm_inputs(70, 3, d, BF16, BF16, "sample", True, True, "cuda", param=BF16)
+
+    def off(t):
+        return torch.cat([t.new_zeros(1), t.reshape(-1)])[1:].view(t.shape)
+
+    w = {k: off(t) for k, t in v.items()}
+    norm_case(w, off(dh), off(ds), "layer", 1.5, True)
+    leaves = {k: t.detach().requires_grad_() for k, t in w.items()}
+
+    def run():
+        h, s = residual_norm(leaves["y"], leaves["x"], leaves["weight"], leaves["bias"], gate=leaves["gate"], post=True,
+                             post_weight=leaves["post_weight"], post_bias=leaves["post_bias"], return_sum=True)
+        return [h, s, *torch.autograd.grad([h, s], list(leaves.values()), [dh, ds])]
+
+    first = run()
+    for _ in range(3):
+        assert all(torch.equal(a, b) for a, b in zip(run(), first))
+
+
 def test_residual_norm_frozen_parts():
     v, dh, _ = norm_inputs(4, 6, 50, BF16, BF16, "channel", True, True, "cuda")
     for k in ("y", "x", "weight", "gate", "post_bias"):
