@@ -35,14 +35,26 @@ struct List {
 template <typename T>
 constexpr int tile_of() { return kTileBytes / (int)sizeof(T); }
 
-__device__ __forceinline__ int find_entry(const List& t, int tile) {
-  int lo = 0, hi = t.n - 1;  // last entry with start <= tile
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (t.start[mid] <= tile) lo = mid; else hi = mid - 1;
+// The table's first tiles, spread over the lanes of a wave, find a tile's entry by ballots: one load's latency for a
+// workgroup, where a binary search in the arguments waits for eight loads in a row for every tile.
+struct Finder {
+  static constexpr int kParts = (kListMax + kWave - 1) / kWave;
+  int start[kParts];
+  __device__ __forceinline__ explicit Finder(const List& t) {
+#pragma unroll
+    for (int k = 0; k < kParts; ++k) {
+      const int e = k * kWave + lane_id();
+      start[k] = e < t.n ? t.start[e] : INT32_MAX;
+    }
   }
-  return lo;
-}
+  // the last entry that starts at the tile or before it
+  __device__ __forceinline__ int operator()(int tile) const {
+    int e = -1;
+#pragma unroll
+    for (int k = 0; k < kParts; ++k) e += __popcll(__ballot(start[k] <= tile));
+    return e;
+  }
+};
 
 template <int P>
 __device__ __forceinline__ double join(double a, double b) {
@@ -89,8 +101,8 @@ __device__ __forceinline__ double tile_norm(const T* __restrict__ p, int n) {
 
 // Calls f(typed pointer, elements) for a tile.
 template <typename F>
-__device__ __forceinline__ void on_tile(const List& t, int tile, F&& f) {
-  const int e = find_entry(t, tile);
+__device__ __forceinline__ void on_tile(const List& t, const Finder& find, int tile, F&& f) {
+  const int e = find(tile);
   const int64_t k = tile - t.start[e], len = t.len[e] & 0x3fffffffu;
   auto go = [&](auto* p) {
     constexpr int64_t T = tile_of<std::remove_pointer_t<decltype(p)>>();
@@ -109,9 +121,12 @@ constexpr int64_t kOnceBytes = 128 << 20;
 template <int P, bool ONCE>
 __global__ __launch_bounds__(kBlock) void norm_part_kernel(List t, double* __restrict__ part) {
   double a = 0.0;
+  const Finder find(t);
   // from the end: whoever reads the gradients next begins at their start, which the memory-side cache still holds
   for (int tile = t.start[t.n] - 1 - (int)blockIdx.x; tile >= 0; tile -= gridDim.x)
-    on_tile(t, tile, [&](auto* p, int n) { a = join<P>(a, tile_norm<std::remove_pointer_t<decltype(p)>, P, ONCE>(p, n)); });
+    on_tile(t, find, tile, [&](auto* p, int n) {
+      a = join<P>(a, tile_norm<std::remove_pointer_t<decltype(p)>, P, ONCE>(p, n));
+    });
   __shared__ double scratch[kBlock / kWave];
   a = block_join<P>(a, scratch);
   if (threadIdx.x == 0) part[blockIdx.x] = a;
@@ -160,8 +175,9 @@ __device__ __forceinline__ void tile_scale(T* __restrict__ p, int n, float f) {
 
 __device__ __forceinline__ void scale_tiles(const List& t, float f) {
   if (f == 1.f) return;
+  const Finder find(t);
   for (int tile = blockIdx.x; tile < t.start[t.n]; tile += gridDim.x)
-    on_tile(t, tile, [&](auto* p, int n) { tile_scale(p, n, f); });
+    on_tile(t, find, tile, [&](auto* p, int n) { tile_scale(p, n, f); });
 }
 
 __global__ __launch_bounds__(kBlock) void scale_kernel(List t, const float* __restrict__ factor) {
