@@ -22,7 +22,9 @@ namespace {
 constexpr int kBlock = 256;
 constexpr int kTileBytes = 16384;
 constexpr int kListMax = 240;    // 3.8 KB of kernel arguments
-constexpr int kMaxBlocks = 1024;  // partial values per launch: four workgroups a CU, 64 KB of loads in flight
+// Partial values per launch: eight workgroups a CU, 128 KB of loads in flight.  Half of them take 79 us for 440 MB, twice
+// as many 67 us, and 9.6 us for 3.9 us to join them.
+constexpr int kMaxBlocks = 2048;
 constexpr int64_t kMaxLen = 1 << 29;  // elements per table entry: longer tensors take several
 
 struct List {
@@ -115,8 +117,9 @@ __device__ __forceinline__ void on_tile(const List& t, const Finder& find, int t
   }
 }
 
-// ONCE: nontemporal loads.  Gradients of 440 MB take 82 us with them and 117 us without, 219 MB 38 and 41 us;
-// 79 MB, which the 256 MB memory-side cache can still hold from the pass that wrote them, 18 and 15 us.
+// Bound by memory.  ONCE: nontemporal loads.  Gradients of 440 MB take 67 us with them (6.6 TB/s) and 72 us without,
+// 219 MB 37 and 40 us; 79 MB, which the 256 MB memory-side cache can still hold from the pass that wrote them, 15.8 and
+// 14.9 us.
 constexpr int64_t kOnceBytes = 128 << 20;
 template <int P, bool ONCE>
 __global__ __launch_bounds__(kBlock) void norm_part_kernel(List t, double* __restrict__ part) {
@@ -185,7 +188,7 @@ __global__ __launch_bounds__(kBlock) void scale_kernel(List t, const float* __re
 }
 
 // With the factor from the partial values; out = nullptr in all launches but the first.  Norm and scaling of 110 million
-// gradients: fp32 250 us (5.3 TB/s of two reads and a write), bf16 115 us (5.8); a factor of one 89 and 40 us.
+// gradients: fp32 209 us (6.3 TB/s of two reads and a write), bf16 112 us (5.9); a factor of one 70 and 38 us.
 template <int P>
 __global__ __launch_bounds__(kBlock) void clip_kernel(List t, const double* __restrict__ part, int64_t n,
                                                       float max_norm, float* __restrict__ out) {
