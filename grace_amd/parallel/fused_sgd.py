@@ -155,7 +155,8 @@ class FusedSGD(SGD):
         bufs = [self.state[p].get("momentum_buffer") for p in params]
         grads = [p.grad for p in params]
         if factor is not None:
-            grads = [(g * factor.to(g.device)).to(g.dtype) for g in grads]
+            # widened by hand: a product of a 16-bit tensor and a device scalar is taken with the scalar in 16 bits
+            grads = [(g.to(factor.dtype) * factor.to(g.device)).to(g.dtype) for g in grads]
         functional_sgd(params, grads, bufs, weight_decay=group["weight_decay"],
                        momentum=group["momentum"], lr=group["lr"], dampening=group["dampening"],
                        nesterov=group["nesterov"], maximize=group.get("maximize", False), foreach=False)
