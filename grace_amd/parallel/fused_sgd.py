@@ -9,7 +9,9 @@ weights=w)`` arranges that automatically.  CPU tensors (and ``GRACE_AMD_FORCE_TO
 
 ``max_grad_norm`` clips by the global norm of all gradients of all groups (parallel/clip.py): the
 update kernel multiplies every gradient by the factor as it reads it, so the gradients themselves stay
-as they are.  The norm of the last step is ``opt.grad_norm`` (a 0-dim device tensor).
+as they are.  The norm of the last step is ``opt.grad_norm`` (a 0-dim device tensor).  The bound is one for
+all groups; like torch's hyper-parameters it is an entry of each of them, so copies, pickles and state dicts
+hold it, and ``opt.max_grad_norm = bound`` changes it.
 
 The learning rate and momentum are read from ``param_groups`` on every ``step()`` call; inside
 a captured HIP graph they are frozen at capture time (as for any host scalar), so LR schedules
@@ -43,18 +45,33 @@ def _same_layout(a: torch.Tensor, b: torch.Tensor) -> bool:
     return a.shape == b.shape and all(sa == sb for sa, sb, n in zip(a.stride(), b.stride(), a.shape) if n > 1)
 
 
+def _checked_bound(bound: Optional[float]) -> Optional[float]:
+    if bound is not None and not bound >= 0:
+        raise ValueError(f"max_grad_norm {bound}: not negative")
+    return bound
+
+
+def _one_bound(groups) -> Optional[float]:
+    bounds = {group.get("max_grad_norm") for group in groups}
+    if len(bounds) > 1:
+        raise ValueError(f"FusedSGD: one max_grad_norm for all groups, not {sorted(bounds, key=str)}")
+    return _checked_bound(bounds.pop()) if bounds else None
+
+
 class FusedSGD(SGD):
-    max_grad_norm: Optional[float] = None
     grad_norm: Optional[torch.Tensor] = None
 
     def __init__(self, params, lr=1e-3, momentum=0.0, dampening=0.0, weight_decay=0.0, nesterov=False, *,
                  maximize: bool = False, max_grad_norm: Optional[float] = None):
-        if max_grad_norm is not None and not max_grad_norm >= 0:
-            raise ValueError(f"max_grad_norm {max_grad_norm}: not negative")
+        _checked_bound(max_grad_norm)
         super().__init__(params, lr=lr, momentum=momentum, dampening=dampening, weight_decay=weight_decay,
                          nesterov=nesterov, maximize=maximize)
         self._working: Dict[int, torch.Tensor] = {}
-        self.max_grad_norm = max_grad_norm
+        for group in self.param_groups:
+            group.setdefault("max_grad_norm", max_grad_norm)
+        if _one_bound(self.param_groups) != max_grad_norm:
+            raise ValueError("FusedSGD: one max_grad_norm for all groups: give it to the optimizer")
+        self.defaults["max_grad_norm"] = max_grad_norm
         # the kernel honours the process-wide communication fault flag (parallel/health.py):
         # allocate it now, before any HIP-graph capture of the step
         devs = {p.device for g in self.param_groups for p in g["params"] if p.is_cuda}
@@ -63,6 +80,31 @@ class FusedSGD(SGD):
 
             for d in sorted(devs, key=lambda d: d.index or 0):
                 health.init(d)
+
+    @property
+    def max_grad_norm(self) -> Optional[float]:
+        return _one_bound(self.param_groups)
+
+    @max_grad_norm.setter
+    def max_grad_norm(self, bound: Optional[float]) -> None:
+        for group in (self.defaults, *self.param_groups):
+            group["max_grad_norm"] = _checked_bound(bound)
+
+    def add_param_group(self, param_group) -> None:
+        if "max_grad_norm" in self.defaults:  # not while the constructor adds its groups
+            _one_bound([self.defaults, {**self.defaults, **param_group}])
+        super().add_param_group(param_group)
+
+    def __setstate__(self, state) -> None:
+        """After load_state_dict (groups without a bound, as torch.optim.SGD's, keep this optimizer's), copies and
+        pickles (whose working copies have to be attached again)."""
+        own = self.__dict__.get("defaults") or state.get("defaults", {})
+        for group in state["param_groups"]:
+            group.setdefault("max_grad_norm", own.get("max_grad_norm"))
+        bound = _one_bound(state["param_groups"])
+        super().__setstate__(state)
+        self.defaults["max_grad_norm"] = bound
+        self.__dict__.setdefault("_working", {})
 
     def attach_working_copies(self, weights) -> None:
         """Write ``weights``' bf16 working copies in the update kernel (BF16Weights)."""

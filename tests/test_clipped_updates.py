@@ -1,5 +1,9 @@
 """Clipping inside the SGD update and over views: 16-bit parameters, copies, pickles and state dicts of the optimizer,
 steps without gradients, gradients that share memory."""
+import copy
+import math
+import pickle
+
 import pytest
 import torch
 import torch.nn as nn
@@ -31,3 +35,71 @@ def test_the_factor_keeps_its_bits(t, device):
         grad = p.grad.double()
         want = -grad * (bound / (grad.norm() + 1e-6))
         O.within(p, want, 3 * O.U * want.abs(), f"{t} {n}")
+
+
+# ---------------------------------------------------------------------------- copies, pickles, state dicts
+def stepped(opt, grads):
+    """The weights after a step with these gradients."""
+    params = [p for group in opt.param_groups for p in group["params"]]
+    for p, g in zip(params, grads):
+        p.grad = g.clone()
+    opt.step()
+    return [p.detach().clone() for p in params]
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("how", ["copy", "pickle"])
+@pytest.mark.parametrize("bound", [0.25, None])
+def test_a_copy_clips_as_its_original(how, bound, device):
+    grads = [torch.full((5,), 2.0, device=device), torch.full((3, 2), -1.0, device=device)]
+    opt = FusedSGD([parameter(g) for g in grads], lr=0.5, momentum=0.9, max_grad_norm=bound)
+    stepped(opt, grads)
+    other = copy.deepcopy(opt) if how == "copy" else pickle.loads(pickle.dumps(opt))
+    assert other.max_grad_norm == bound
+    for a, b in zip(stepped(opt, grads), stepped(other, grads)):
+        assert torch.equal(a, b)
+
+
+def test_state_dicts_hold_the_bound():
+    grads = [torch.full((5,), 2.0)]
+
+    def made(cls=FusedSGD, **kw):
+        return cls([parameter(g) for g in grads], lr=0.5, momentum=0.9, **kw)
+
+    opt = made(max_grad_norm=0.25)
+    stepped(opt, grads)
+    plain = made()
+    plain.load_state_dict(opt.state_dict())
+    assert plain.max_grad_norm == 0.25
+    opt.load_state_dict(made(max_grad_norm=0.5).state_dict())
+    assert opt.max_grad_norm == 0.5
+    # torch's optimizer loads it, and its state dict, which has no bound, leaves the one that there is
+    ref = made(torch.optim.SGD)
+    ref.load_state_dict(opt.state_dict())
+    opt.load_state_dict(made(torch.optim.SGD).state_dict())
+    assert opt.max_grad_norm == 0.5
+    opt.load_state_dict(made().state_dict())
+    assert opt.max_grad_norm is None
+
+
+def test_one_bound_for_all_groups():
+    a, b, c = (parameter(torch.full((4,), 3.0)) for _ in range(3))
+    opt = FusedSGD([{"params": [a]}, {"params": [b], "lr": 0.1}], lr=1.0, max_grad_norm=1.0)
+    opt.add_param_group({"params": [c]})
+    opt.step()
+    assert abs(float(opt.grad_norm) - 108 ** 0.5) < 1e-5
+    opt.max_grad_norm = 2.0
+    assert opt.max_grad_norm == 2.0 and all(group["max_grad_norm"] == 2.0 for group in opt.param_groups)
+    for bad in (-1.0, math.nan):
+        with pytest.raises(ValueError):
+            opt.max_grad_norm = bad
+    assert opt.max_grad_norm == 2.0
+    with pytest.raises(ValueError):
+        opt.add_param_group({"params": [parameter(torch.ones(2))], "max_grad_norm": 1.0})
+    with pytest.raises(ValueError):
+        FusedSGD([{"params": [a], "max_grad_norm": 1.0}, {"params": [b]}], lr=1.0)
+    state = opt.state_dict()
+    state["param_groups"][1]["max_grad_norm"] = 1.0
+    with pytest.raises(ValueError):
+        opt.load_state_dict(state)
+    assert opt.max_grad_norm == 2.0
