@@ -9,11 +9,12 @@ weights=w)`` arranges that automatically.  CPU tensors (and ``GRACE_AMD_FORCE_TO
 
 ``max_grad_norm`` clips by the global norm of all gradients of all groups (parallel/clip.py): the
 update kernel multiplies every gradient by the factor as it reads it, so the gradients themselves stay
-as they are.  The norm of the last step is ``opt.grad_norm`` (a 0-dim device tensor).  The bound is one for
-all groups; like torch's hyper-parameters it is an entry of each of them, so copies, pickles and state dicts
-hold it, and ``opt.max_grad_norm = bound`` changes it.
+as they are.  The norm of the last step is ``opt.grad_norm``: a 0-dim device tensor, zero in a step
+without gradients, None in one without a bound.  The bound is one for all groups; like torch's
+hyper-parameters it is an entry of each of them, so copies, pickles and state dicts hold it, and
+``opt.max_grad_norm = bound`` changes it.
 
-The learning rate and momentum are read from ``param_groups`` on every ``step()`` call; inside
+The learning rate, momentum and bound are read from ``param_groups`` on every ``step()`` call; inside
 a captured HIP graph they are frozen at capture time (as for any host scalar), so LR schedules
 need eager steps or a re-capture.
 """
@@ -120,7 +121,9 @@ class FusedSGD(SGD):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        factor = self._clip_factor() if self.max_grad_norm is not None else None
+        bound = self.max_grad_norm
+        self.grad_norm = None
+        factor = self._clip_factor(float(bound)) if bound is not None else None
         for group in self.param_groups:
             native, rest = [], []
             on = {}  # device -> whether its native path runs
@@ -143,20 +146,21 @@ class FusedSGD(SGD):
                 self._torch_step(group, rest, factor)
         return loss
 
-    def _clip_factor(self) -> Optional[torch.Tensor]:
+    def _clip_factor(self, bound: float) -> Optional[torch.Tensor]:
         from .clip import _check, _norm_and_factor, _unique
 
         params = [p for g in self.param_groups for p in g["params"]]
         if _native.use_native(params[0]):
-            out = _native.lib().grad_clip(params, 2, float(self.max_grad_norm), False)
+            out = _native.lib().grad_clip(params, 2, bound, False)
             if out is not None:
                 self.grad_norm = out[0]
                 return out[1]
         grads = _unique([p.grad for p in params if p.grad is not None])
         if not grads:
+            self.grad_norm = torch.zeros((), device=params[0].device)
             return None
         _check(grads)
-        self.grad_norm, factor = _norm_and_factor(grads, 2, float(self.max_grad_norm))
+        self.grad_norm, factor = _norm_and_factor(grads, 2, bound)
         return factor
 
     def _native_step(self, group, params, factor):

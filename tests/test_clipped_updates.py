@@ -103,3 +103,23 @@ def test_one_bound_for_all_groups():
     with pytest.raises(ValueError):
         opt.load_state_dict(state)
     assert opt.max_grad_norm == 2.0
+
+
+# ---------------------------------------------------------------------------- steps without gradients
+@pytest.mark.parametrize("device", DEVICES)
+def test_the_norm_is_the_last_steps(device):
+    p = parameter(torch.ones(3, device=device))
+    opt = FusedSGD([p], lr=0.1, max_grad_norm=1.0)
+    opt.step()
+    assert abs(float(opt.grad_norm) - 3 ** 0.5) < 1e-6
+    opt.zero_grad(set_to_none=True)
+    before = p.detach().clone()
+    opt.step()
+    assert opt.grad_norm.shape == () and opt.grad_norm.device == p.device and float(opt.grad_norm) == 0.0
+    assert torch.equal(p, before)
+    p.grad = torch.full((3,), 2.0, device=device)
+    opt.step()
+    assert abs(float(opt.grad_norm) - 12 ** 0.5) < 1e-6
+    opt.max_grad_norm = None  # an unclipped step takes no norm
+    opt.step()
+    assert opt.grad_norm is None
