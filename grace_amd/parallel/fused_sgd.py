@@ -150,14 +150,14 @@ class FusedSGD(SGD):
         from .clip import _check, _norm_and_factor, _unique
 
         params = [p for g in self.param_groups for p in g["params"]]
-        if _native.use_native(params[0]):
+        if params and _native.use_native(params[0]):
             out = _native.lib().grad_clip(params, 2, bound, False)
             if out is not None:
                 self.grad_norm = out[0]
                 return out[1]
         grads = _unique([p.grad for p in params if p.grad is not None])
         if not grads:
-            self.grad_norm = torch.zeros((), device=params[0].device)
+            self.grad_norm = torch.zeros((), device=params[0].device if params else None)
             return None
         _check(grads)
         self.grad_norm, factor = _norm_and_factor(grads, 2, bound)

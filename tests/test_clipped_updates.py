@@ -123,3 +123,15 @@ def test_the_norm_is_the_last_steps(device):
     opt.max_grad_norm = None  # an unclipped step takes no norm
     opt.step()
     assert opt.grad_norm is None
+
+
+def test_a_step_without_parameters():
+    opt = FusedSGD([{"params": []}], lr=0.1, max_grad_norm=1.0)
+    opt.step()
+    assert float(opt.grad_norm) == 0.0
+    p = parameter(torch.full((4,), 2.0))
+    opt.add_param_group({"params": [p]})
+    opt.step()
+    assert float(opt.grad_norm) == 4.0
+    want = torch.full((4,), -0.1 * 2.0 / (4.0 + 1e-6), dtype=F64)
+    O.within(p, want, 8 * O.U * want.abs())  # lr, factor and two products
