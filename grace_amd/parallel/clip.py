@@ -49,9 +49,49 @@ def _native_ok(g: torch.Tensor) -> bool:
     return g.dtype in _DTYPES and _native.use_native(g)
 
 
+def _memory(g: torch.Tensor):
+    """Equal for two tensors that show the same elements, in whatever order."""
+    if g.layout != torch.strided or g.numel() == 0:
+        return id(g)
+    places = (g.numel(),) if _dense(g) else tuple(sorted((s, n) for s, n in zip(g.stride(), g.shape) if n > 1))
+    return g.device, g.data_ptr(), g.dtype, places
+
+
+def _apart(grads: List[torch.Tensor]) -> bool:
+    """No two of these tensors, some with gaps between their elements, share any of their memory."""
+    unit = min(g.element_size() for g in grads)
+    base = min(g.data_ptr() for g in grads)
+    shown = torch.zeros((max(_end(g) for g in grads) - base) // unit, dtype=torch.int16)
+    for g in grads:
+        k = g.element_size() // unit
+        shown.as_strided((*g.shape, k), (*(s * k for s in g.stride()), 1), (g.data_ptr() - base) // unit).add_(1)
+    return int(shown.max()) <= 1
+
+
+def _end(g: torch.Tensor) -> int:
+    return g.data_ptr() + (1 + sum(s * (n - 1) for s, n in zip(g.stride(), g.shape))) * g.element_size()
+
+
+def _expanded(g: torch.Tensor) -> bool:
+    return any(s == 0 and n > 1 for s, n in zip(g.stride(), g.shape))
+
+
 def _unique(grads: List[torch.Tensor]) -> List[torch.Tensor]:
-    """Every tensor once: a repeated one counts once and is scaled once."""
-    return list({id(g): g for g in grads}.values())
+    """Every piece of memory once: one that several tensors show counts once and is scaled once, as in the kernels'
+    own list.  Tensors that share a part of their memory are refused."""
+    once = list({_memory(g): g for g in grads}.values())
+    by = {}
+    for g in once:
+        if g.layout == torch.strided and g.numel() > 0 and not _expanded(g):
+            by.setdefault(g.device, []).append(g)
+    for on in by.values():
+        run, end = [], 0  # tensors whose spans of memory meet
+        for g in sorted(on, key=lambda g: g.data_ptr()):
+            run = run + [g] if g.data_ptr() < end else [g]
+            end = max(end, _end(g))
+            if len(run) > 1 and (all(_dense(t) for t in run) or not _apart(run)):
+                raise RuntimeError("gradient norm: two tensors overlap")
+    return once
 
 
 def _groups(grads: List[torch.Tensor]):
@@ -115,7 +155,7 @@ def _scale(grads: List[torch.Tensor], factor: torch.Tensor) -> None:
 def _grads_of(parameters) -> List[torch.Tensor]:
     grads = _unique([p.grad for p in parameters if p.grad is not None])
     _check(grads)
-    if any(s == 0 and n > 1 for g in grads for s, n in zip(g.stride(), g.shape)):
+    if any(_expanded(g) for g in grads):
         raise ValueError("clip_grad_norm_: an expanded gradient: several of its elements share memory")
     return grads
 
@@ -123,7 +163,8 @@ def _grads_of(parameters) -> List[torch.Tensor]:
 @torch.no_grad()
 def grad_norm(tensors: Iterable[torch.Tensor], norm_type: float = 2.0) -> torch.Tensor:
     """The norm of all tensors taken as one vector: a 0-dim tensor (fp32; fp64 if any tensor is) on the
-    first tensor's device.  ``norm_type``: 1, 2 or inf.  A tensor that is given twice counts once."""
+    first tensor's device.  ``norm_type``: 1, 2 or inf.  Memory that is given twice, by the same tensor or by
+    two views of all its elements, counts once; tensors that share a part of theirs are refused."""
     tensors = [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
     kind, tensors = _kind(norm_type), _unique(tensors)
     _check(tensors)
@@ -136,9 +177,10 @@ def grad_norm(tensors: Iterable[torch.Tensor], norm_type: float = 2.0) -> torch.
 def clip_grad_norm_(parameters: Union[torch.Tensor, Iterable[torch.Tensor]], max_norm: float, norm_type: float = 2.0,
                     error_if_nonfinite: bool = False) -> torch.Tensor:
     """Scale the parameters' ``.grad`` in place by ``min(1, max_norm / (norm + 1e-6))`` and return the norm
-    before it (0-dim).  ``norm_type``: 1, 2 or inf.  A shared parameter counts once.  A non-finite
-    norm makes the gradients NaN or zero, as torch's function does; ``error_if_nonfinite`` raises instead,
-    before anything is scaled, for which it waits for the device."""
+    before it (0-dim).  ``norm_type``: 1, 2 or inf.  A shared parameter or gradient counts once, also as two
+    views; gradients that share a part of their memory are refused.  A non-finite norm makes the gradients NaN or
+    zero, as torch's function does; ``error_if_nonfinite`` raises instead, before anything is scaled, for
+    which it waits for the device."""
     kind, max_norm = _kind(norm_type), float(max_norm)
     if not max_norm >= 0:
         raise ValueError(f"max_norm {max_norm}: not negative")
