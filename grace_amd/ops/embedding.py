@@ -19,13 +19,23 @@ import torch.nn.functional as F
 
 from . import _native
 
+
+def _plain(ids, weight, scale, padding_idx, dtype):
+    """With rows of NaN, and no gradient, for tokens outside the table."""
+    wide = weight if weight.dtype == torch.float64 else weight.float()
+    inside = (ids >= 0) & (ids < weight.shape[0])
+    y = F.embedding(torch.where(inside, ids, 0), wide, padding_idx) * float(scale)
+    return torch.where(inside[..., None], y, float("nan")).to(dtype)
+
+
 def embedding(ids: torch.Tensor, weight: torch.Tensor, scale: float = 1.0, padding_idx: Optional[int] = None,
               dtype: Optional[torch.dtype] = None) -> torch.Tensor:
     """``round(scale * weight[ids])`` of shape ``[*ids.shape, width]``.
 
     ``ids``: int64 or int32, any shape and strides.  ``weight``: ``[rows, width]``, float32, bfloat16 or
-    float16, on a GPU at most 2^21 wide.  ``dtype``: the output's type (default: the table's).  ``padding_idx`` (negative: from the end)
-    names a row that gets no gradient.  Differentiable once, in ``weight``."""
+    float16, on a GPU at most 2^21 wide.  ``dtype``: the output's type (default: the table's).
+    ``padding_idx`` (negative: from the end) names a row that gets no gradient.  Differentiable once, in
+    ``weight``."""
     if _native.use_native(weight):
         return _native.lib().embedding(ids, weight, scale, padding_idx, dtype)  # the same refusals, in C++
     if ids.dtype not in (torch.int64, torch.int32):
@@ -39,8 +49,11 @@ def embedding(ids: torch.Tensor, weight: torch.Tensor, scale: float = 1.0, paddi
         raise ValueError("embedding: the table has no rows")
     if padding_idx is not None and not -rows <= padding_idx < rows:
         raise ValueError(f"embedding: padding_idx {padding_idx} outside a table of {rows} rows")
+    out = weight.dtype if dtype is None else dtype
+    if weight.is_cuda and rows > 0:  # without the kernels: what they give, and torch reads nothing behind the table
+        return _plain(ids, weight, scale, padding_idx, out)
     wide = weight if weight.dtype == torch.float64 else weight.float()
-    return (F.embedding(ids, wide, padding_idx) * float(scale)).to(weight.dtype if dtype is None else dtype)
+    return (F.embedding(ids, wide, padding_idx) * float(scale)).to(out)
 
 
 class ScaledEmbedding(nn.Embedding):
