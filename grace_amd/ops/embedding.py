@@ -33,7 +33,7 @@ def embedding(ids: torch.Tensor, weight: torch.Tensor, scale: float = 1.0, paddi
     """``round(scale * weight[ids])`` of shape ``[*ids.shape, width]``.
 
     ``ids``: int64 or int32, any shape and strides.  ``weight``: ``[rows, width]``, float32, bfloat16 or
-    float16, on a GPU at most 2^21 wide.  ``dtype``: the output's type (default: the table's).
+    float16 (on the CPU float64 too), on a GPU at most 2^21 wide.  ``dtype``: the output's type (default: the table's).
     ``padding_idx`` (negative: from the end) names a row that gets no gradient.  Differentiable once, in
     ``weight``."""
     if _native.use_native(weight):
@@ -50,6 +50,9 @@ def embedding(ids: torch.Tensor, weight: torch.Tensor, scale: float = 1.0, paddi
     if padding_idx is not None and not -rows <= padding_idx < rows:
         raise ValueError(f"embedding: padding_idx {padding_idx} outside a table of {rows} rows")
     out = weight.dtype if dtype is None else dtype
+    for t in (weight.dtype, out):
+        if t not in (torch.float32, torch.bfloat16, torch.float16, torch.float64):
+            raise TypeError(f"embedding: float32, bfloat16 or float16, got {weight.dtype} -> {out}")
     if weight.is_cuda and rows > 0:  # without the kernels: what they give, and torch reads nothing behind the table
         return _plain(ids, weight, scale, padding_idx, out)
     wide = weight if weight.dtype == torch.float64 else weight.float()

@@ -46,3 +46,14 @@ def test_plain_form_of_tokens_outside_the_table(pad):
     O.within(dw, rdw, dwb, "dw")
     with pytest.raises(IndexError):
         embedding(ids, w)
+
+
+# ---------------------------------------------------------------------------- types
+@pytest.mark.parametrize("device", DEVICES)
+def test_embedding_refuses_other_types(device):
+    ids, w = torch.tensor([1, 0], device=device), torch.ones(3, 4, device=device)
+    for table, out in ((w.long(), None), (w.bool(), F32), (w, torch.int32), (w, torch.bool), (w.to(torch.complex64), None)):
+        with pytest.raises(TypeError):
+            embedding(ids, table, dtype=out)
+    if device == "cpu":
+        assert embedding(ids, w.double(), 0.5).dtype == F64 and embedding(ids, w, dtype=F64).dtype == F64
