@@ -162,6 +162,9 @@ constexpr int kSortWaves = 16;
 constexpr int kSortBlock = kSortWaves * kWave;
 constexpr int kSmall = kSortBlock * 8;   // pairs that one workgroup sorts in LDS
 constexpr int kManyTiles = 64;           // tiles of 2048 pairs before they grow to 8192
+// Up to so many tiles each adds up all tiles' counts itself, work that grows with their square: 4 million tokens (512
+// tiles, 8 columns) 1042 us and 1045 with a scan of the counts in a launch of its own, 17 million (2048) 1838 and 1451.
+constexpr int kScanTiles = 512;
 
 // Memory that a launch clears with the workgroups behind its own: bytes [begin, end) of p (16-byte aligned).
 struct Fill {
@@ -312,14 +315,45 @@ __global__ __launch_bounds__(kSortBlock) void sort_count_kernel(EmbedIds ids, in
   if (threadIdx.x < kRadix) count[(int64_t)blockIdx.x * kRadix + threadIdx.x] = hist[threadIdx.x];
 }
 
-// Moves one tile's pairs to their places; each workgroup adds up the tiles' counts itself.  (Counting the next
-// pass's digits here saves a launch and loses more: a token that fills an eighth of the batch sends as many
-// atomics to one address, 42 us for 65536 tokens.)
+// Of many tiles the counts become places once, a workgroup for each digit: count[tile][digit] turns into the sum over the
+// tiles before it, and the row behind the tiles into the digits' totals.
+__global__ __launch_bounds__(kSortBlock) void sort_scan_kernel(int tiles, uint32_t* __restrict__ count) {
+  __shared__ uint32_t waves[kSortWaves];
+  const int w = wave_id();
+  uint32_t* at = count + blockIdx.x;
+  uint32_t base = 0;
+  for (int t0 = 0; t0 < tiles; t0 += kSortBlock) {
+    const int t = t0 + threadIdx.x;
+    const uint32_t v = t < tiles ? at[(int64_t)t * kRadix] : 0u;
+    uint32_t s = v;
+#pragma unroll
+    for (int o = 1; o < kWave; o <<= 1) {
+      const uint32_t u = __shfl_up(s, o, kWave);
+      if (lane_id() >= o) s += u;
+    }
+    __syncthreads();  // the last round's sums have been read
+    if (lane_id() == kWave - 1) waves[w] = s;
+    __syncthreads();
+    uint32_t before = 0, all = 0;
+#pragma unroll
+    for (int i = 0; i < kSortWaves; ++i) {
+      if (i < w) before += waves[i];
+      all += waves[i];
+    }
+    if (t < tiles) at[(int64_t)t * kRadix] = base + before + s - v;
+    base += all;
+  }
+  if (threadIdx.x == 0) at[(int64_t)tiles * kRadix] = base;
+}
+
+// Moves one tile's pairs to their places; each workgroup adds up the tiles' counts itself, or finds the sums there
+// (scanned).  (Counting the next pass's digits here saves a launch and loses more: a token that fills an eighth of the
+// batch sends as many atomics to one address, 42 us for 65536 tokens.)
 template <int PER>
 __global__ __launch_bounds__(kSortBlock) void sort_move_kernel(EmbedIds ids, int tiles,
                                                                const uint32_t* __restrict__ in_key,
                                                                const uint32_t* __restrict__ in_val, int shift,
-                                                               const uint32_t* __restrict__ count,
+                                                               const uint32_t* __restrict__ count, bool scanned,
                                                                uint32_t* __restrict__ out_key,
                                                                uint32_t* __restrict__ out_val, Fill fill) {
   if ((int)blockIdx.x >= tiles) return fill_zero(fill, blockIdx.x - tiles, gridDim.x - tiles);
@@ -339,11 +373,18 @@ __global__ __launch_bounds__(kSortBlock) void sort_move_kernel(EmbedIds ids, int
   }
   uint32_t before = 0, total = 0;
   const int q = tid & (kRadix - 1), group = tid / kRadix;
+  if (scanned) {
+    if (group == 0) {
+      before = count[(int64_t)blockIdx.x * kRadix + q];
+      total = count[(int64_t)tiles * kRadix + q];
+    }
+  } else {
 #pragma unroll 4
-  for (int i = group; i < tiles; i += kSortBlock / kRadix) {
-    const uint32_t c = count[(int64_t)i * kRadix + q];
-    if (i < (int)blockIdx.x) before += c;
-    total += c;
+    for (int i = group; i < tiles; i += kSortBlock / kRadix) {
+      const uint32_t c = count[(int64_t)i * kRadix + q];
+      if (i < (int)blockIdx.x) before += c;
+      total += c;
+    }
   }
   sums[0][group][q] = before;
   sums[1][group][q] = total;
@@ -375,7 +416,7 @@ struct Runs {
   const uint32_t* val;  // the tokens in that order
   int64_t n;
   uint32_t vocab;
-  int chunk;            // sorted tokens per chunk: 8 to 64, a power of two
+  int chunk;            // sorted tokens per chunk: 8, 16 or 32
   float* head;  // [chunks, d]: the part of a run that began in an earlier chunk
   float* tail;  // [chunks, d]: the part of a run that begins here and goes on
   uint32_t* joins;      // their number, and then the chunks where such runs begin, in any order
@@ -389,7 +430,7 @@ __global__ __launch_bounds__(kBlock) void run_sum_kernel(Runs a, const TD* __res
                                                          TG* __restrict__ dw) {
   constexpr int V = vec_of<TD, float>(), kSlab = kWave * V;
   constexpr int U = 8;  // rows in flight
-  const int64_t c = (int64_t)blockIdx.x * kWaves + wave_id();
+  const int64_t c = ((int64_t)blockIdx.z * gridDim.x + blockIdx.x) * kWaves + wave_id();
   const int64_t begin = c * a.chunk;
   if (begin >= a.n) return;
   const int cnt = (int)min((int64_t)a.chunk, a.n - begin);
@@ -574,7 +615,7 @@ int64_t embed_backward_ws(int64_t n, int64_t vocab, int64_t d) {
   if (n <= kFew) return 0;
   const Plan p = plan_of(n);
   return 4 * align256(4 * n) + 2 * align256(4 * p.chunks * d) + align256(4 * (p.chunks + 1)) +
-         (n > kSmall ? align256((int64_t)4 * p.tiles * kRadix) : 0);
+         (n > kSmall ? align256((int64_t)4 * (p.tiles + 1) * kRadix) : 0);
 }
 
 void embed_backward(const EmbedIds& ids, const void* dy, ElType tdy, int64_t d, float scale, void* dw, ElType tdw,
@@ -587,7 +628,8 @@ void embed_backward(const EmbedIds& ids, const void* dy, ElType tdy, int64_t d, 
       by_type(tdy, [&](auto* tag_d) {
         using TD = std::remove_pointer_t<decltype(tag_d)>;
         const int64_t slabs = cdiv(d, kWave * vec_of<TD, float>());
-        // about 64 KB to clear for a workgroup: the ids that it reads for it are at most an eighth of that
+        // 64 KB to clear for a workgroup, but no more than kClearRows rows and no less than one; of rows of 64 bytes
+        // and more the ids that it reads for it, 8 KB at most, are an eighth of that
         const int64_t each = std::max<int64_t>(1, std::min<int64_t>(kClearRows, 65536 / (d * (int64_t)sizeof(TG))));
         int log = 0;
         while (log < 8 && ((int64_t)(16 / sizeof(TG)) << log) < d) ++log;
@@ -620,16 +662,18 @@ void embed_backward(const EmbedIds& ids, const void* dy, ElType tdy, int64_t d, 
                                                                        Fill{dw, 0, bytes});
       return;
     }
-    uint32_t* count = (uint32_t*)take((int64_t)4 * plan.tiles * kRadix);
+    uint32_t* count = (uint32_t*)take((int64_t)4 * (plan.tiles + 1) * kRadix);
     const int64_t share = align256(cdiv(bytes, 2 * passes));  // of the fill, for each launch
     auto fill = [&](int k) { return Fill{dw, std::min(k * share, bytes), std::min((k + 1) * share, bytes)}; };
     const unsigned grid = plan.tiles + kFillBlocks;
+    const bool scanned = plan.tiles > kScanTiles;
     for (int p = 0; p < passes; ++p) {
       const uint32_t *ik = p ? key[now] : nullptr, *iv = p ? val[now] : nullptr;
       now = p & 1;
       sort_count_kernel<PER><<<grid, kSortBlock, 0, stream>>>(ids, plan.tiles, ik, 8 * p, count, joins, fill(2 * p));
-      sort_move_kernel<PER><<<grid, kSortBlock, 0, stream>>>(ids, plan.tiles, ik, iv, 8 * p, count, key[now], val[now],
-                                                            fill(2 * p + 1));
+      if (scanned) sort_scan_kernel<<<kRadix, kSortBlock, 0, stream>>>(plan.tiles, count);
+      sort_move_kernel<PER><<<grid, kSortBlock, 0, stream>>>(ids, plan.tiles, ik, iv, 8 * p, count, scanned, key[now],
+                                                            val[now], fill(2 * p + 1));
     }
   });
   const Runs runs{key[now], val[now], n, (uint32_t)ids.vocab, plan.chunk, head, tail, joins};
@@ -638,7 +682,9 @@ void embed_backward(const EmbedIds& ids, const void* dy, ElType tdy, int64_t d, 
     by_type(tdy, [&](auto* tag_d) {
       using TD = std::remove_pointer_t<decltype(tag_d)>;
       const unsigned slabs = (unsigned)cdiv(d, kWave * vec_of<TD, float>());
-      const dim3 grid((unsigned)cdiv(plan.chunks, kWaves), slabs);
+      // a dimension of a grid holds less than 2^32 threads
+      const int64_t blocks = cdiv(plan.chunks, kWaves), x = std::min<int64_t>(blocks, 1 << 23);
+      const dim3 grid((unsigned)x, slabs, (unsigned)cdiv(blocks, x));
       if (n * d * (int64_t)sizeof(TD) >= kOnceBytes)
         run_sum_kernel<TD, TG, true><<<grid, kBlock, 0, stream>>>(runs, (const TD*)dy, d, scale, (TG*)dw);
       else

@@ -57,3 +57,38 @@ def test_embedding_refuses_other_types(device):
             embedding(ids, table, dtype=out)
     if device == "cpu":
         assert embedding(ids, w.double(), 0.5).dtype == F64 and embedding(ids, w, dtype=F64).dtype == F64
+
+
+# ---------------------------------------------------------------------------- very many tokens
+@pytest.mark.gpu
+@pytest.mark.parametrize("n,vocab,d,out,index", [
+    (4300007, 1 << 24, 1, F32, torch.int32),  # counts scanned in a launch of their own, four passes
+    (4300007, 257, 5, F16, torch.int64)])
+def test_gradient_of_many_tokens(n, vocab, d, out, index):
+    g = torch.Generator("cuda").manual_seed(0)
+    ids = torch.randint(0, vocab, (n,), generator=g, device="cuda")
+    ids[torch.rand(n, generator=g, device="cuda") < 0.1] = vocab - 1  # a run over many chunks
+    ids[::1001] = -1
+    ids[n // 2] = vocab
+    w = torch.zeros(vocab, d, device="cuda", requires_grad=True)
+    flat = torch.randn(n * d + 1, generator=g, device="cuda").to(out)
+    dy = flat[1:].view(n, d)  # one element behind an aligned address
+    pad = 7
+    y = embedding(ids.to(index), w, 1.5, pad, out)
+    dw, = torch.autograd.grad(y, w, dy)
+    _, _, want, bound = O.embedding(ids.cpu(), w.detach().cpu(), 1.5, pad, dy.cpu())
+    O.within(dw.cpu(), want, bound, "dw")
+    again, = torch.autograd.grad(embedding(ids.to(index), w, 1.5, pad, out), w, dy)
+    assert torch.equal(dw, again)
+
+
+@pytest.mark.gpu
+def test_gradient_of_the_most_tokens():
+    """2^31 - 2 tokens: every row's sum of ones is a whole number below 2^24, which fp32 holds in any order."""
+    n, vocab = 2**31 - 2, 300
+    ids = torch.arange(n, device="cuda", dtype=torch.int32).remainder_(vocab)
+    w = torch.zeros(vocab, 1, device="cuda", requires_grad=True)
+    y = embedding(ids, w, dtype=F16)
+    dw, = torch.autograd.grad(y, w, torch.ones(n, 1, dtype=F16, device="cuda"))
+    want = n // vocab + (torch.arange(vocab, device="cuda") < n % vocab).long()
+    assert torch.equal(dw[:, 0].double(), want.double())
