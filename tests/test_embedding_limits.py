@@ -62,6 +62,8 @@ def test_embedding_refuses_other_types(device):
 # ---------------------------------------------------------------------------- very many tokens
 @pytest.mark.gpu
 @pytest.mark.parametrize("n,vocab,d,out,index", [
+    (131073, 70000, 3, F32, torch.int64),    # eight pairs to a thread of the sort, over three passes
+    (140001, 300, 481, BF16, torch.int64),   # 128 MB and more of gradients, read past the caches, at odd addresses
     (4300007, 1 << 24, 1, F32, torch.int32),  # counts scanned in a launch of their own, four passes
     (4300007, 257, 5, F16, torch.int64)])
 def test_gradient_of_many_tokens(n, vocab, d, out, index):
@@ -80,6 +82,21 @@ def test_gradient_of_many_tokens(n, vocab, d, out, index):
     O.within(dw.cpu(), want, bound, "dw")
     again, = torch.autograd.grad(embedding(ids.to(index), w, 1.5, pad, out), w, dy)
     assert torch.equal(dw, again)
+
+
+@pytest.mark.gpu
+def test_sorted_gradient_of_far_rows():
+    """A gradient of more than 2^31 elements whose tokens are sorted, and its last rows."""
+    vocab, d, n = 2**20 + 5, 2100, 3000
+    g = torch.Generator("cuda").manual_seed(1)
+    rows = torch.tensor([0, 3, 2**20 - 1, 2**20, 2**20 + 4], device="cuda")
+    at = torch.randint(0, 5, (n,), generator=g, device="cuda")
+    w = torch.zeros(vocab, d, dtype=BF16, device="cuda", requires_grad=True)
+    dy = torch.randn(n, d, generator=g, device="cuda").to(BF16)
+    dw, = torch.autograd.grad(embedding(rows[at], w), w, dy)
+    _, _, want, bound = O.embedding(at, torch.zeros(5, d, device="cuda"), 1.0, None, dy)
+    O.within(dw[rows], want, bound, "dw")
+    assert int(dw.any(1).sum()) == 5
 
 
 @pytest.mark.gpu
