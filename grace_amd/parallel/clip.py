@@ -13,6 +13,9 @@ In data-parallel training the norm is that of the exchanged gradients, the same 
     with opt.skip_synchronize():
         opt.step()
 
+(With :class:`~grace_amd.parallel.precision.BF16Weights` the exchanged gradients are those of
+``weights.master_parameters(model)``; the model's own parameters hold the local ones.)
+
 ``FusedSGD(..., max_grad_norm=1.0)`` does the same inside its update, without writing the clipped
 gradients.
 """
