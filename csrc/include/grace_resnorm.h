@@ -21,8 +21,10 @@
 // partial row; a second launch adds the partial rows in a fixed order.
 //
 // Bound by memory: a copy runs at 5.2 TB/s.  64 million values in whole vectors, forward and backward: bf16 widths of
-// 64 to 16384 at 4.7-5.5 and 4.0-4.4 TB/s, fp32 at 4.7-5.5 and 4.1-4.9.  With a norm behind the block and a gate: up to
-// 8192 columns 4.4-5.5 and 3.1-4.9, wider ones 3.8-4.2 and, for want of registers, 2.5 (bf16) and 4.2 (fp32).
+// 64 to 16384 at 4.7-5.5 and 4.0-4.4 TB/s, fp32 at 4.7-5.5 and 4.1-4.9.  With a norm behind the block and a gate, rms and
+// without biases: up to 8192 columns 4.4-5.5 and 3.1-4.9, wider ones 3.8-4.2 and, for want of registers, 2.5 (bf16) and
+// 4.2 (fp32).  With both biases more registers are short: up to 8192 columns 3.5-5.4 and 2.9-4.8 in whole vectors, 12000
+// columns 3.1-3.3 and 0.8 (bf16) and 1.8 (fp32).  An fp32 stream with a bf16 block up to 8192 columns: 4.9-5.6 and 4.4-4.6.
 #pragma once
 
 #include <algorithm>
@@ -381,8 +383,9 @@ struct ParamPlaces {
   }
 };
 
-// Forward: at most five arrays in LDS, 80 KB; 1024 threads would take 160 KB and have registers enough.  fp32 rows of 16
-// values a thread take them from the caches, when their sums are done: 4096 rows of 768 take 10.4 us and 11.3 with LDS,
+// Forward: at most five arrays in LDS, 80 KB; 1024 threads would take 160 KB.  Theirs are in registers, of which 8 values a
+// thread take 82 to 97; with 16 values 128 do not hold them, and 60 to 186 are spilled (12000 columns, all five arrays: 3.3
+// TB/s in bf16, 3.1 in fp32).  fp32 rows of 16 values a thread take them from the caches, when their sums are done: 4096 rows of 768 take 10.4 us and 11.3 with LDS,
 // which is filled before the first row; in 16 bits (64 million values in rows of 650) 3.6 TB/s and 4.4 with LDS.
 template <typename TY, int E, int TPR>
 constexpr Home forward_home() {
@@ -527,7 +530,9 @@ __device__ __forceinline__ void over_slots(const float (&acc)[J][V], const Row<T
 }
 
 // BIAS: one of the two biases is there.  Four waves to a SIMD hold 128 registers each: a few of them spilled cost less
-// than the fourth wave (fp32, 1536 columns, gate and post norm: 332 us, 362 us with three waves of 131 registers).
+// than the fourth wave (fp32, 1536 columns, gate and post norm: 332 us, 362 us with three waves of 131 registers).  Single
+// values in rows of 512 threads, odd widths of 2049 to 4095, pay more for it: 63 to 199 registers are spilled (bf16, 3001
+// columns: 3.3 TB/s, with gate, post norm and biases 1.2).
 template <typename TX, typename TY, int E, int TPR, int V, bool POST, bool GATED, bool BIAS>
 __global__ __launch_bounds__(block_of<TPR>(),
                              TPR == 512 || (TPR == 256 && V > 1) ? 4 : 1) void resnorm_bwd_kernel(BwdArgs g) {
@@ -788,6 +793,8 @@ void launch_backward(const BwdArgs& a, hipStream_t stream) {
       kernel<<<(unsigned)a.split.blocks, block_of<TPR>(), lds, stream>>>(a);
     });
   };
+  // a form without biases for whole vectors only (16 bf16 values for each of 64 threads, gate and post norm: 209
+  // registers, two waves to a SIMD; with biases 266 and one)
   auto by_bias = [&](auto post, auto gated) {
     by_vec<TY>(a.n.d, [&](auto v) {
       if constexpr (decltype(v)::value == vec_of<TY>())

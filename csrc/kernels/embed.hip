@@ -99,7 +99,8 @@ __device__ __forceinline__ void clear_rows(const EmbedIds& ids, int64_t r0, int6
 // Workgroup (token t, slab of columns), and behind those the ones that clear.  Each wave looks through a quarter of
 // the tokens and notes those of t's row; if t is the first of them the waves sum their notes and meet in LDS
 // in token order.  700 tokens of 650 fp32 columns into 10000 rows: 12.6 us for 28 MB, the latency of a search, a sum
-// and a meeting one after the other (sorting takes three launches).
+// and a meeting one after the other, and of the clearing behind them, which starts when the token workgroups have been
+// dispatched (sorting takes three launches).
 template <typename TD, typename TG>
 __global__ __launch_bounds__(kBlock) void embed_few_kernel(EmbedIds ids, const TD* __restrict__ dy, int64_t d,
                                                            float scale, TG* __restrict__ dw, int slabs, int rows_each,

@@ -59,8 +59,8 @@ def residual_norm(y: torch.Tensor, residual: Optional[torch.Tensor] = None, weig
     ``residual``: the stream, of y's shape, of its type or float32.  ``weight``, ``bias``, ``post_weight``,
     ``post_bias``: ``[width]``; ``gate``: ``[width]``, or y's shape with 1 in place of trailing dimensions
     before the last (``[batch, 1, width]``: one gate a sample); each float32 or of y's type.  ``alpha``
-    scales the residual and has no gradient.  Tensors that are not contiguous are copied first.
-    Differentiable once."""
+    scales the residual and has no gradient.  Without a residual, a gate and ``post``, ``s`` is ``y``, not a
+    copy.  Tensors that are not contiguous are copied first.  Differentiable once."""
     if _native.use_native(y):  # the same refusals, in C++
         out = _native.lib().residual_norm(y, residual, weight, bias, kind, eps, gate, alpha, post, post_weight,
                                           post_bias, return_sum)

@@ -1,7 +1,7 @@
 """The global gradient norm over many tensors, and clipping by it (``csrc/kernels/gradnorm.hip``).
 
-``clip_grad_norm_`` has the interface and the formula of ``torch.nn.utils.clip_grad_norm_``:
-gradients are multiplied by ``min(1, max_norm / (norm + 1e-6))``.  The norm is summed in fp64 over all
+``clip_grad_norm_`` has the formula of ``torch.nn.utils.clip_grad_norm_`` and its arguments but for
+``foreach``, with 1, 2 and inf for ``norm_type``: gradients are multiplied by ``min(1, max_norm / (norm + 1e-6))``.  The norm is summed in fp64 over all
 tensors, whatever their types, in one launch per 240 tensors and in a fixed order; nothing waits for
 the host, so the call can be captured into a HIP graph.  A factor of one leaves the gradients' memory
 untouched.
