@@ -88,11 +88,15 @@ def _unique(grads: List[torch.Tensor]) -> List[torch.Tensor]:
         if g.layout == torch.strided and g.numel() > 0 and not _expanded(g):
             by.setdefault(g.device, []).append(g)
     for on in by.values():
-        run, end = [], 0  # tensors whose spans of memory meet
+        runs, end = [], 0  # tensors whose spans of memory meet
         for g in sorted(on, key=lambda g: g.data_ptr()):
-            run = run + [g] if g.data_ptr() < end else [g]
+            if g.data_ptr() < end:
+                runs[-1].append(g)
+            else:
+                runs.append([g])
             end = max(end, _end(g))
-            if len(run) > 1 and (all(_dense(t) for t in run) or not _apart(run)):
+        for run in runs:
+            if len(run) > 1 and (all(_dense(g) for g in run) or not _apart(run)):
                 raise RuntimeError("gradient norm: two tensors overlap")
     return once
 
