@@ -52,6 +52,17 @@ class _DistributedOptimizer:
     def __getattr__(self, item):
         return getattr(self._opt, item)
 
+    # an assignment would stay with the wrapper otherwise
+    @property
+    def max_grad_norm(self):
+        return self._opt.max_grad_norm
+
+    @max_grad_norm.setter
+    def max_grad_norm(self, bound):
+        if not hasattr(self._opt, "max_grad_norm"):
+            raise AttributeError(f"{type(self._opt).__name__} does not clip: call clip_grad_norm_ between synchronize and step")
+        self._opt.max_grad_norm = bound
+
     def synchronize(self):
         self.engine.synchronize()
         self._synchronized = True

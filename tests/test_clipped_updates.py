@@ -191,3 +191,27 @@ def test_overlapping_gradients_are_refused(raises, device):
         with pytest.raises(RuntimeError, match="overlap"):
             clip_grad_norm_(pair, 1.0, error_if_nonfinite=raises)
     assert torch.equal(flat, torch.ones_like(flat))
+
+
+# ---------------------------------------------------------------------------- the wrapped optimizer
+def test_the_bound_through_the_distributed_optimizer():
+    from grace_amd import grace_from_params
+    from grace_amd.parallel import DistributedOptimizer
+
+    def wrapped(cls, **kw):
+        p = nn.Parameter(torch.zeros(4))
+        opt = DistributedOptimizer(cls([p], lr=1.0, **kw), grace_from_params(
+            {"compressor": "none", "memory": "none", "communicator": "allreduce", "world_size": 1}))
+        (p * torch.full((4,), 2.0)).sum().backward()
+        return p, opt
+
+    p, opt = wrapped(FusedSGD, max_grad_norm=8.0)
+    assert opt.max_grad_norm == 8.0
+    opt.max_grad_norm = 1.0
+    opt.step()
+    want = torch.full((4,), -2.0 / (4.0 + 1e-6), dtype=F64)
+    O.within(p, want, 4 * O.U * want.abs())
+    _, plain = wrapped(torch.optim.SGD)
+    for call in (lambda: plain.max_grad_norm, lambda: setattr(plain, "max_grad_norm", 1.0)):
+        with pytest.raises(AttributeError):
+            call()
