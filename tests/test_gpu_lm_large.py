@@ -107,3 +107,27 @@ def test_clipped_update_past_the_caches(kw, bound):
         for p, r in zip(ps, ref):
             O.within(p, r.detach(), 12 * O.U * (step + 1) * (r.detach().abs() + 0.4 * (step + 1) * p.grad.abs() * f))
     assert torch.equal(flat[:3], edge)
+
+
+def test_the_most_rows():
+    """2^31 - 2 rows of one value.  The rms norm of +-1 with eps = 0 is +-1 in fp32, so with weight 2 and bias 1 h is 3 or
+    -1, and dweight and dbias are whole numbers."""
+    n = 2**31 - 2
+    y = torch.ones(n, 1, dtype=BF16, device="cuda")
+    y[1::2] = -1.0
+    w = torch.full((1,), 2.0, device="cuda", requires_grad=True)
+    b = torch.full((1,), 1.0, device="cuda", requires_grad=True)
+    h = residual_norm(y, None, w, b, kind="rms", eps=0.0)
+    assert bool((h.view(-1, 2) == torch.tensor([3.0, -1.0], dtype=BF16, device="cuda")).all())
+    dh = torch.zeros(n, 1, dtype=BF16, device="cuda")
+    dh[::2], dh[-3:] = 1.0, 4.0
+    dw, db = torch.autograd.grad(h, [w, b], dh)
+    # the last three rows have 4 each, two of them with y = -1; sums of whole numbers, each rounded at most 40 times
+    ones = n // 2 - 1
+    assert abs(float(db) - (ones + 12)) <= 40 * O.U * (ones + 12)
+    assert abs(float(dw) - (ones + 4 - 8)) <= 40 * O.U * (ones + 12)
+    # and with whole numbers below 2^24 exactly
+    dh.zero_()
+    dh[::1024], dh[-3:] = 1.0, 4.0
+    dw, db = torch.autograd.grad(residual_norm(y, None, w, b, kind="rms", eps=0.0), [w, b], dh)
+    assert float(db) == n // 1024 + 1 + 12 and float(dw) == n // 1024 + 1 + 4 - 8
